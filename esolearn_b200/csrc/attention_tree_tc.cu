@@ -48,6 +48,7 @@
 #include <type_traits>
 
 #include "attention_tree_dev.cuh"
+#include "clock_pace.cuh"
 #include "tcgen05.cuh"
 
 namespace sb {
@@ -760,10 +761,17 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
         const uint32_t id_s = idesc_f16(TT_TILE, DT == SB_KV_BF16, false), id_o = idesc_f16(HD, DT == SB_KV_BF16, true);
         // Products are issued no faster than they run (64 clocks; 32 for head_dim 64's second one): a product that waits
         // for the tensor cores holds up the barrier polls of the softmax warps beside this one (2000 clocks a tile).
-        clock_t pace_from = 0;
+        // The wait, of at most 62 * 21 clocks, is bounded twice: by the clock, whose differences are taken modulo its 2^32,
+        // and by the number of readings.
+        auto clock32 = []() {
+            uint32_t c;
+            asm volatile("mov.u32 %0, %%clock;" : "=r"(c)::"memory");
+            return c;
+        };
+        uint32_t pace_from = 0;
         auto pace = [&](int n) {
             if ((n & 3) == 3)
-                while (clock() - pace_from < 62 * (n - 2)) {
+                for (int i = 0; i < 1024 && !clocks_passed(pace_from, clock32(), 62 * (n - 2)); i++) {
                 }
         };
         for (int t = 0; t <= nt && ok; t++) {
@@ -774,7 +782,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
                 if (ok && t >= C::NSB) ok = mbar_wait_long(pv_done + 8 * buf, (t / C::NSB - 1) & 1);
                 if (!ok) break;
                 tc_fence_after();
-                pace_from = clock();
+                pace_from = clock32();
                 const uint64_t kd = sw128_desc(base + stage * C::STAGE + MAT, 16);
 #pragma unroll
                 for (int q = QT - 1; q >= 0; q--) {  // small terms first: less is cut off
@@ -794,7 +802,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
                 ok = mbar_wait_long(v_full + 8 * stage, ((t - 1) / NS) & 1) && mbar_wait_long(p_full + 8 * buf, ((t - 1) / C::NSB) & 1);
                 if (!ok) break;
                 tc_fence_after();
-                pace_from = clock();
+                pace_from = clock32();
                 const uint64_t vd = sw128_desc(base + stage * C::STAGE, 16384);
 #pragma unroll
                 for (int q = 1; q >= 0; q--)

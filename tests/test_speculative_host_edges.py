@@ -1,0 +1,28 @@
+"""Speculative decoding, host side: what kernels and wrappers have to hold at the edges of their arguments (no GPU)."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "esolearn_b200", "csrc")
+
+
+@pytest.fixture(scope="module")
+def pace(tmp_path_factory):
+    """clocks_passed of the kernels' pacing loop, compiled for the host."""
+    d = tmp_path_factory.mktemp("pace")
+    src, lib = d / "pace.cpp", d / "libpace.so"
+    src.write_text('#include "clock_pace.cuh"\nextern "C" int passed(uint32_t a, uint32_t b, uint32_t n) { return sb::clocks_passed(a, b, n); }\n')
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I" + CSRC, "-o", str(lib), str(src)], check=True)
+    f = C.CDLL(str(lib)).passed
+    f.argtypes, f.restype = [C.c_uint32] * 3, C.c_int
+    return f
+
+
+@pytest.mark.parametrize("start", [0, 1, 2 ** 31 - 30, 2 ** 31, 2 ** 32 - 1000, 2 ** 32 - 62, 2 ** 32 - 1])
+@pytest.mark.parametrize("n", [62, 62 * 13])
+def test_pacing_ends_across_the_counters_wrap(pace, start, n):
+    """Read every 20 clocks from `start` on, the wait is over at the first reading n clocks later, and stays over."""
+    for dt in range(0, 4 * n, 20):
+        assert bool(pace(start, (start + dt) % 2 ** 32, n)) == (dt >= n)
