@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
     pdl_launch_dependents();  // the join's blocks wait for this kernel's end
     int *s_bad = reinterpret_cast<int *>(sm + C::BAR_OFF + 216);  // [2] bf16: a tail tile's V holds non-finite elements
     float(*s_svmax)[TT_LOADERS] = reinterpret_cast<float(*)[TT_LOADERS]>(sm + C::BAR_OFF + 224);  // int8: largest finite |v_scale|
-    static_assert(TT_LOADERS == 3 && TT_SCALES * 8 + 136 <= 208 && 224 + TT_SCALES * TT_LOADERS * 4 <= 328, "barriers and small words");
+    static_assert(C::NS == 2 && TT_LOADERS == 3 && TT_SCALES * 8 + 136 <= 208 && 224 + TT_SCALES * TT_LOADERS * 4 <= 328, "barriers and small words");
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int nkv = a.c.pg.n_kv;
@@ -219,7 +219,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
     const uint32_t s_full = bars, p_full = bars + 24, pv_done = bars + 48;  // [3]: of tile t at t % NSB
     const uint32_t k_full = bars + 72, v_full = bars + 88;  // [2]: at t % NS
     const uint32_t sc_full = bars + 136;  // [TT_SCALES]
-    const uint32_t q_full = bars + 336, tail_full = bars + 344;
+    const uint32_t q_full = bars + 336;
+    // [2]: V of tail tile t has landed, at t % NS.  One barrier for both stages would not do: a loader may lag a whole tile
+    // behind the one that issues the copies, whose next phase would then hide the one that it waits for.
+    const uint32_t tail_full = bars + 104;
     const uint32_t raw_k = bars + 352, raw_v = bars + 400;  // [TT_LOADERS][2], [4]
     if (tid == 0) {
         for (int i = 0; i < 3; i++) {
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
         }
         for (int i = 0; i < TT_SCALES; i++) mbar_init(sc_full + 8 * i, TT_LOADERS);
         mbar_init(q_full, TT_SOFTMAX_WARPS);
-        mbar_init(tail_full, 1);
+        for (int i = 0; i < 2; i++) mbar_init(tail_full + 8 * i, 1);
         for (int i = 0; i < 2 * TT_LOADERS; i++) mbar_init(raw_k + 8 * i, 1);
         for (int i = 0; i < 4; i++) mbar_init(raw_v + 8 * i, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -665,7 +668,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
             const int box = a.box_rows;
             int2 rows = make_int2(-1, -1);
             unsigned hand = 0;  // steps whose arrival follows their copies, newest in bit 0
-            int tails = 0;
+            unsigned tail_phase = 0;  // of tail_full, a bit per stage
             // row of this lane's box of a tile, looked up a tile ahead
             const int part = lane / (HD / 64), blk = lane % (HD / 64);
             auto box_row = [&](int t) {
@@ -687,7 +690,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
                     if (ok && box > 0) {
                         if (lw == 0) {
                             if (!isv) y_next = box_row(t + 1);
-                            const uint32_t bar = tail ? tail_full : full;
+                            const uint32_t bar = tail ? tail_full + 8 * stage : full;
                             if (lane == 0) mbar_expect_tx(bar, MAT);
                             __syncwarp();
                             if (part * box < TT_TILE) tma_box(smem_u32(dst) + blk * 16384 + part * box * 128, isv ? &a.tmv : &a.tmk, blk * 64, y, bar);
@@ -715,10 +718,10 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
                     if (ok && tail) {
                         // A non-finite V element of a drafted row must not reach rows that do not see it (0 * inf): it is a
                         // zero in the product, and the sums add it where it is seen.
-                        if (box > 0) wait(tail_full, tails & 1);
+                        if (box > 0) wait(tail_full + 8 * stage, (tail_phase >> stage) & 1);
                         else cp_wait<0>();
                         __syncwarp();
-                        tails++;
+                        tail_phase ^= 1u << stage;
                         bool bad = false;
 #pragma unroll 4
                         for (int i = 0; i < TT_GROUPS * NI; i++) {
