@@ -167,6 +167,9 @@ __global__ void __launch_bounds__(VT, 1) verify_kernel(const VerifyArgs a, int t
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
+    // A CTA's shared memory may be written by another only once it has started: all arrive here and wait, with the first
+    // row's copy and the tree's tables between, before the first exchange.
+    if (cs > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     unsigned phase[2] = {0, 0};
     // starts the copy of a node's row (its 16-byte part) into buffer `buf`; thread 0
     auto start = [&](int n, int buf) {
@@ -223,6 +226,7 @@ __global__ void __launch_bounds__(VT, 1) verify_kernel(const VerifyArgs a, int t
         }
     }
     __syncthreads();
+    if (cs > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 
     auto cluster_sync = [&]() {
         if (cs > 1) cl.sync();

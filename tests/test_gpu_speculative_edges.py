@@ -6,7 +6,7 @@ import pytest
 
 import esolearn_b200 as E
 from esolearn_b200 import _native as N
-from test_gpu_speculative import IO, check_attention, gen, make_cache, ref_attention, seen_of
+from test_gpu_speculative import IO, check_attention, check_verify, gen, make_cache, noise_of, ref_attention, seen_of
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -37,3 +37,27 @@ def test_chains_over_many_tiles_of_drafted_rows(kv, io, hd, page, ctx):
     check_attention(out, ref_attention(q, cache, [ctx], seen_of(t)), io)
     for _ in range(50):
         assert torch.equal(out, E.tree_attention(q, cache, cl, ctx + t))
+
+
+# ---------------------------------------------------------------------------
+# verification
+
+@pytest.mark.parametrize("b,n,v,temp", [(1, 1, 8192, 1.0), (2, 1, 33000, 0.9), (64, 1, 8196, 1.0), (18, 2, 32771, 0.0), (1, 1, 400001, 0.7)])
+def test_short_walks_of_several_ctas(b, n, v, temp):
+    # one row a sequence, split over a cluster: the CTAs' first exchange comes soon after their start
+    g = gen(b + v)
+    logits = torch.randn(b, n, v, generator=g, device="cuda") * 2
+    tokens = torch.zeros(b, n, dtype=torch.int32, device="cuda")
+    parents = torch.arange(-1, n - 1, dtype=torch.int32, device="cuda")
+    if temp == 0.0:
+        best = logits.argmax(-1)
+        tokens[:, 1:] = best[:, :-1].int()
+        path, keep, nxt = E.verify_drafts(logits, tokens, parents, temperature=temp)
+        assert keep.tolist() == [n] * b and torch.equal(nxt.long(), best[:, -1])
+        return
+    u = torch.rand(b, n, generator=g, device="cuda")
+    noise = noise_of(g, b, v)
+    first = check_verify(logits, tokens, parents, u, noise, temp)
+    for _ in range(100):
+        again = E.verify_drafts(logits, tokens, parents, u, noise, temperature=temp)
+        assert all(torch.equal(x, y) for x, y in zip(first, again))
