@@ -88,6 +88,15 @@ def _rows(t, name: str):
     return t, h * d
 
 
+def _matrix_rows(x):
+    """(tensor, row stride) of a [B, V] tensor with contiguous rows; a copy where rows overlap, such as one row expanded
+    over the batch."""
+    b, v = x.shape
+    if b <= 1:
+        return x, v
+    return (x, x.stride(0)) if x.stride(0) >= v else (x.contiguous(), v)
+
+
 class KvCache:
     """A paged K/V cache: k and v [pages, n_kv, page_size, head_dim] of bfloat16, float32 or int8 (int8: codes with
     one float32 scale per row in k_scale, v_scale [pages, n_kv, page_size]) and the page table [B, max_pages] int32.
@@ -269,7 +278,8 @@ def verify_drafts(logits, tokens, parents, u=None, noise=None, temperature: floa
     if noise is not None:
         if noise.dtype is not torch.float32 or noise.device != dev or noise.shape != (b, v) or not (noise.stride(1) == 1 or v == 1):
             raise N.SbError(_SHAPE, f"verify_drafts: noise must be float32 ({b}, {v})")
-        np_, nl = noise.data_ptr(), max(noise.stride(0), v)
+        noise, nl = _matrix_rows(noise)
+        np_ = noise.data_ptr()
     pld = n if parents.dim() == 2 else 0
     tp = _ints(tokens, (b, n), "verify_drafts: tokens", dev)
     path, n_accept = torch.empty_like(tokens), tokens.new_empty((b,))

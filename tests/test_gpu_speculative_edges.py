@@ -6,7 +6,7 @@ import pytest
 
 import esolearn_b200 as E
 from esolearn_b200 import _native as N
-from test_gpu_speculative import IO, check_attention, check_verify, gen, make_cache, noise_of, ref_attention, seen_of
+from test_gpu_speculative import IO, check_attention, check_verify, gen, make_cache, noise_of, ref_attention, ref_verify, seen_of
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -61,3 +61,24 @@ def test_short_walks_of_several_ctas(b, n, v, temp):
     for _ in range(100):
         again = E.verify_drafts(logits, tokens, parents, u, noise, temperature=temp)
         assert all(torch.equal(x, y) for x, y in zip(first, again))
+
+
+@pytest.mark.parametrize("b,v", [(3, 1000), (1, 1000), (4, 33001)])
+@pytest.mark.parametrize("draft", [False, True])
+def test_noise_shared_by_the_batch(b, v, draft):
+    # one row of noise expanded over the sequences, and rows that overlap, are what their copies are
+    g = gen(v)
+    logits = torch.randn(b, 3, v, generator=g, device="cuda") * 2
+    q = torch.softmax(logits + 0.5 * torch.randn(b, 3, v, generator=g, device="cuda"), -1) if draft else None
+    tokens = logits.argmax(-1).roll(1, 1).int().contiguous()
+    parents = ints([-1, 0, 1])
+    u = torch.rand(b, 3, generator=g, device="cuda")
+    one = noise_of(g, 1, v + 16)
+    for noise in (one[:, :v].expand(b, v), one.as_strided((b, v), (4, 1))):
+        got = E.verify_drafts(logits, tokens, parents, u, noise, draft_probs=q)
+        want = E.verify_drafts(logits, tokens, parents, u, noise.contiguous(), draft_probs=q)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        for i in range(b):
+            path, tok, near = ref_verify(logits[i], tokens[i], parents.tolist(), u[i], noise[i], 1.0, None if q is None else q[i])
+            if near > 1e-4:
+                assert got[0][i].tolist() == path + [-1] * (3 - len(path)) and int(got[2][i]) == tok

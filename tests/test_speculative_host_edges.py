@@ -4,6 +4,9 @@ import os
 import subprocess
 
 import pytest
+import torch
+
+from esolearn_b200 import speculative as S
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "esolearn_b200", "csrc")
 
@@ -26,3 +29,16 @@ def test_pacing_ends_across_the_counters_wrap(pace, start, n):
     """Read every 20 clocks from `start` on, the wait is over at the first reading n clocks later, and stays over."""
     for dt in range(0, 4 * n, 20):
         assert bool(pace(start, (start + dt) % 2 ** 32, n)) == (dt >= n)
+
+
+@pytest.mark.parametrize("make", [lambda x: x[:1].expand(3, 7), lambda x: x.flatten().as_strided((3, 7), (5, 1)), lambda x: x, lambda x: x[:, :6],
+                                  lambda x: x[:1, :5], lambda x: x[::2], lambda x: x[:0]])
+def test_rows_of_a_matrix_stay_inside_its_storage(make):
+    """Row i of what a kernel is given lies at i times the stride, within the tensor's memory, and holds row i."""
+    x = make(torch.arange(21.0).view(3, 7))
+    y, ld = S._matrix_rows(x)
+    b, v = x.shape
+    assert ld >= v
+    last = y.storage_offset() + (b - 1) * ld + v
+    assert b == 0 or last <= y.untyped_storage().nbytes() // 4
+    assert torch.equal(torch.as_strided(y, (b, v), (ld, 1)), x)
