@@ -10,9 +10,9 @@ token, nodes 1..N-1 are drafted, node i under node parents[i] < i.
     ctx_len += n_accept                                               # `token` is the next step's node 0
 
 N = 1 is plain decoding.  The calls run on torch's current stream and wait for
-nothing; every one goes to libscryb200.so (declarations and the exact rules in
-include/sb_api.h).  The reference decodes one token per step from an f32 cache
-and has no counterpart.
+nothing; their tensors lie on the thread's current device.  Every call goes to
+libscryb200.so (declarations and the exact rules in include/sb_api.h).  The
+reference decodes one token per step from an f32 cache and has no counterpart.
 """
 from __future__ import annotations
 
@@ -31,17 +31,21 @@ def _need(ok: bool, message: str, code: int = _SHAPE) -> None:
         raise N.SbError(code, message)
 
 
-_raw_stream = None
+_raw_stream = _raw_device = None
 
 
 def _stream(t) -> int:
-    """The current stream of t's device (the raw handle: torch.cuda.current_stream builds an object, 2 us a call)."""
-    global _raw_stream
+    """The current stream of t's device, which has to be the thread's current device: the library launches there (raw
+    handle and number: torch.cuda.current_stream builds an object, 2 us a call)."""
+    global _raw_stream, _raw_device
     if _raw_stream is None:
         import torch
 
+        _raw_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
         _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
-    i = t.get_device()
+    i, here = t.get_device(), _raw_device()
+    if i != here:
+        raise N.SbError(_ARG, f"tensors on cuda:{i}, but the current device is cuda:{here} (torch.cuda.device({i}) makes theirs current)")
     return _raw_stream(i)
 
 

@@ -6,6 +6,7 @@ import subprocess
 import pytest
 import torch
 
+from esolearn_b200 import _native as N
 from esolearn_b200 import speculative as S
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "esolearn_b200", "csrc")
@@ -42,3 +43,23 @@ def test_rows_of_a_matrix_stay_inside_its_storage(make):
     last = y.storage_offset() + (b - 1) * ld + v
     assert b == 0 or last <= y.untyped_storage().nbytes() // 4
     assert torch.equal(torch.as_strided(y, (b, v), (ld, 1)), x)
+
+
+class _On:
+    """Stands for a tensor on a device."""
+
+    def __init__(self, device):
+        self.device = device
+
+    def get_device(self):
+        return self.device
+
+
+def test_tensors_of_another_device_are_refused(monkeypatch):
+    """The library launches on the thread's current device: a stream of another one must not reach it."""
+    monkeypatch.setattr(S, "_raw_stream", lambda i: 1000 + i)
+    monkeypatch.setattr(S, "_raw_device", lambda: 1, raising=False)
+    assert S._stream(_On(1)) == 1001
+    for other in (0, 2):
+        with pytest.raises(N.SbError, match=f"cuda:{other}"):
+            S._stream(_On(other))
