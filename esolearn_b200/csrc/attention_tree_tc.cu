@@ -7,7 +7,8 @@
 // sums of 16-bit terms, accumulated in TMEM:
 //   int8 cache: the codes as exact f16; q (over a power of two of its row's
 //     magnitude) as two f16 terms (one when q is bf16); k_scale multiplies the
-//     scores; p * v_scale as two f16 terms;
+//     scores; p * v_scale, over a power of two of the largest that the row sees,
+//     as two f16 terms;
 //   bf16 cache: K and V as they are, q as three bf16 terms (one when q is
 //     bf16), p as two.
 // Each tile's O starts from zero and is added to the row's sums in registers in
@@ -67,7 +68,9 @@ constexpr int tt_regs_softmax(int dt, bool bf16) { return dt != SB_KV_I8 && bf16
 constexpr int tt_regs_sums(int dt) { return dt == SB_KV_I8 ? 160 : 152; }
 constexpr int tt_regs_rest(int dt, bool bf16) { return 4 * 128 - 2 * tt_regs_softmax(dt, bf16) - tt_regs_sums(dt); }
 constexpr int TT_GROUPS = (16 + TT_LOADERS - 1) / TT_LOADERS;  // groups of eight positions of a tile that a loader has
-constexpr int TT_SCALES = 8;  // tiles whose scales are kept
+constexpr int TT_SCALES = 4;  // tiles whose scales are kept
+// p * v_scale * 2^kw, the weights' f16 terms, is below 2^TT_KW when kw is chosen and at most 2^TT_KW_MAX while it serves.
+constexpr float TT_KW = 7.0f, TT_KW_MAX = 14.0f;
 
 template <int HD, int DT, bool BF16>
 struct TtShape {
@@ -83,9 +86,9 @@ struct TtShape {
     // int8: codes as they come: two runs (tiles) for every loader's groups of K, one for every sums warp's of V
     static constexpr int RAWK = TT_GROUPS * 8 * HD, RAWV = 4 * 8 * HD;
     static constexpr int RAW_OFF = Q_OFF + (QTMEM ? 0 : QT * MAT);
-    static constexpr int SC_OFF = RAW_OFF + (DT == SB_KV_I8 ? TT_LOADERS * 2 * RAWK + 4 * RAWV : 0);  // int8: [TT_SCALES][k scale, v scale][128]
-    static constexpr int SC_BYTES = DT == SB_KV_I8 ? TT_SCALES * 2 * 128 * 4 : 0;
-    static constexpr int EX_OFF = SC_OFF + SC_BYTES;  // [2][2][128]: row maxima of the halves; int8: of v_scale too
+    static constexpr int SC_OFF = RAW_OFF + (DT == SB_KV_I8 ? TT_LOADERS * 2 * RAWK + 4 * RAWV : 0);  // int8: [TT_SCALES][k scale, v scale, log2 v scale][128]
+    static constexpr int SC_BYTES = DT == SB_KV_I8 ? TT_SCALES * 3 * 128 * 4 : 0;
+    static constexpr int EX_OFF = SC_OFF + SC_BYTES;  // [2][2][128]: row maxima of the halves; int8: of log2(p * v_scale) too
     static constexpr int AL_OFF = EX_OFF + 2 * 2 * 128 * (DT == SB_KV_I8 ? 8 : 4);  // [4][128] bytes: log2 of the sums' rescaling
     static constexpr int BAR_OFF = AL_OFF + 4 * 128;
     static constexpr int BYTES = BAR_OFF + 448;
@@ -205,8 +208,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
     uint32_t &s_tmem = *reinterpret_cast<uint32_t *>(sm + C::BAR_OFF + 208);
     pdl_launch_dependents();  // the join's blocks wait for this kernel's end
     int *s_bad = reinterpret_cast<int *>(sm + C::BAR_OFF + 216);  // [2] bf16: a tail tile's V holds non-finite elements
-    float(*s_svmax)[TT_LOADERS] = reinterpret_cast<float(*)[TT_LOADERS]>(sm + C::BAR_OFF + 224);  // int8: largest finite |v_scale|
-    static_assert(C::NS == 2 && TT_LOADERS == 3 && TT_SCALES * 8 + 136 <= 208 && 224 + TT_SCALES * TT_LOADERS * 4 <= 328, "barriers and small words");
+    static_assert(C::NS == 2 && TT_LOADERS == 3 && TT_SCALES * 8 + 136 <= 208, "barriers and small words");
 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int nkv = a.c.pg.n_kv;
@@ -404,8 +406,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
         if (lane == 0) mbar_arrive(q_full);
     }
 
-    float m = -INFINITY, l = 0.0f;  // softmax: weights are 2^(score - m + kw), m whole
-    int kw = 0;
+    float m = -INFINITY, l = 0.0f, kw = 0.0f;  // softmax: weights are 2^(score - m + kw), m and kw whole
     // A wait that gives up (2 s) ends all later ones of its warp; the warps still go through their loops, so that no
     // barrier between warps is left waiting.
     bool ok = true;
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
 #pragma unroll
                 for (int j = 0; j < 32; j++) s[j] = pack2(x[j >> 4][(j & 15) * 2], x[j >> 4][(j & 15) * 2 + 1]);
             }
-            const float *sc = reinterpret_cast<const float *>(sm + C::SC_OFF) + (t % TT_SCALES) * 256 + half * 64;
+            const float *sc = reinterpret_cast<const float *>(sm + C::SC_OFF) + (t % TT_SCALES) * 384 + half * 64;
             if (DT == SB_KV_I8) {
 #pragma unroll
                 for (int j = 0; j < 32; j += 2) {
@@ -467,39 +468,41 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
                 }
                 top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
             }
-            // int8: the largest v_scale that the row sees in this tile
-            float vtop = 0.0f;
+            // int8: the largest log2(2^score |v_scale|) of what the row sees in this tile, to within one
+            float wtop = -INFINITY;
             if (DT == SB_KV_I8) {
-                const float *x = s_svmax[t % TT_SCALES];
-                vtop = max3(x[0], x[1], x[2]);
-                if (tail) {
-                    vtop = 0.0f;
-                    for (int j = 0; j < 64; j++)
-                        if ((vis >> j) & 1) {
-                            const float y = fabsf(sc[128 + j]);
-                            if (y < INFINITY) vtop = fmaxf(vtop, y);
-                        }
+                float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < 32; j += 2) {
+                    const ulonglong2 v4 = *reinterpret_cast<const ulonglong2 *>(sc + 256 + 2 * j);
+                    const float2 x = unpack2(fma2(s[j], f2, v4.x)), y = unpack2(fma2(s[j + 1], f2, v4.y));
+                    m4[j & 2] = max3(m4[j & 2], x.x, x.y), m4[(j & 2) + 1] = max3(m4[(j & 2) + 1], y.x, y.y);
                 }
+                wtop = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
             }
             // the row's other half; behind this barrier both have their scores in registers
             ex[(buf * 2 + half) * 128 + rl] = top;
-            if (DT == SB_KV_I8) exw[(buf * 2 + half) * 128 + rl] = vtop;
+            if (DT == SB_KV_I8) exw[(buf * 2 + half) * 128 + rl] = wtop;
             pair_sync(1 + quad);
             top = fmaxf(top, ex[(buf * 2 + (half ^ 1)) * 128 + rl]) * f;
-            if (DT == SB_KV_I8) vtop = fmaxf(vtop, exw[(buf * 2 + (half ^ 1)) * 128 + rl]);
+            if (DT == SB_KV_I8) wtop = fmaxf(wtop, exw[(buf * 2 + (half ^ 1)) * 128 + rl]);
             const float m_old = m;
-            const int kw_old = kw;
+            const float kw_old = kw;
             if (top > m + 8.0f) m = ceilf(top);
-            if (DT == SB_KV_I8) {
-                // p <= 2^8 and |v_scale| < 2^(e + 1), so p * v_scale * 2^kw < 2^15
-                const int e = min(max((int)(__float_as_uint(vtop) >> 23) - 127, -90), 106);
-                if (m_old == -INFINITY || kw > 6 - e) kw = 6 - e;
+            if (DT == SB_KV_I8 && m > -INFINITY) {
+                // kw keeps p * v_scale * 2^kw in f16's range, by what the row sees and what weight it gives it: a large
+                // scale of little weight costs the others nothing.  It rises with m, by which older weights have shrunk, and
+                // is chosen anew where this tile's weights would leave the range.  (Rows that see nothing here: wtop -inf.)
+                const float e = ceilf(wtop - m);
+                if (m_old > -INFINITY) kw += m - m_old;
+                if (m_old == -INFINITY || kw + e > TT_KW_MAX) kw = TT_KW - e;
+                kw = fminf(fmaxf(kw, -100.0f), 96.0f);
             }
             // (2^-127 and less is as good as nothing; ex2 gives 0)
-            const float la = m_old == -INFINITY ? -127.0f : fmaxf((m_old - m) + (float)(kw - kw_old), -127.0f);
+            const float la = m_old == -INFINITY ? -127.0f : fmaxf((m_old - m) + (kw - kw_old), -127.0f);
             const float alpha = la > -127.0f ? ex2(la) : 0.0f;
             if (half == 0) al[(t & 3) * 128 + rl] = (signed char)la;
-            const float off = m == -INFINITY ? 0.0f : (float)kw - m;
+            const float off = m == -INFINITY ? 0.0f : kw - m;
             const uint64_t off2 = pack2(off, off);
             uint64_t l2 = pack2(0.0f, 0.0f);
             auto weights = [&](auto masked) {
@@ -632,18 +635,16 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
             for (int t = 0; t < nt; t++) {
                 const int stage = t % NS, slot = t % TT_SCALES;
                 if (t >= NS) wait(s_full + 8 * ((t - NS) % C::NSB), ((t - NS) / C::NSB) & 1);
-                // (the scales in this slot, of tile t-8, have been read: q K^T of t-2 came after p V of t-5)
-                float *sc = reinterpret_cast<float *>(sm + C::SC_OFF) + slot * 256 + (lane & 7);
-                float vtop = 0.0f;
+                // (the scales in this slot, of tile t-4, have been read: p V of t-4, which waits for all of its weights, was
+                // issued before q K^T of t-2)
+                float *sc = reinterpret_cast<float *>(sm + C::SC_OFF) + slot * 384 + (lane & 7);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const int grp = lw + (h * 4 + (lane >> 3)) * TT_LOADERS;
                     const float k1 = h ? sk.y : sk.x, v1 = h ? sv.y : sv.x;
-                    if (grp < 16) sc[grp * 8] = k1, sc[128 + grp * 8] = v1;
-                    if (fabsf(v1) < INFINITY) vtop = fmaxf(vtop, fabsf(v1));
+                    const int e = (int)(__float_as_uint(v1) << 1 >> 24);  // |v1| < 2^(e - 126); what is not finite reaches its output anyhow
+                    if (grp < 16) sc[grp * 8] = k1, sc[128 + grp * 8] = v1, sc[256 + grp * 8] = e == 255 ? -150.0f : (float)(e - 126);
                 }
-                vtop = warp_max_f(vtop);
-                if (lane == 0) s_svmax[slot][lw] = vtop;
                 fetch_scales(r1);
                 r2 = look_up(t + 2);
                 wait(bar + 8 * (t & 1), (t >> 1) & 1);
@@ -830,7 +831,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
     // ---- the output or the splits' join
     if (warp < TT_SOFTMAX_WARPS) ex[half * 128 + rl] = l;
     __syncthreads();
-    if (warp < 4) rm[rl] = m == -INFINITY ? m : m - (float)kw, rs[rl] = ex[rl] + ex[128 + rl];
+    if (warp < 4) rm[rl] = m == -INFINITY ? m : m - kw, rs[rl] = ex[rl] + ex[128 + rl];
     __syncthreads();
     const size_t tile = ((size_t)b * nkv + g) * (gridDim.x / a.n_splits) + rt;
     tree_finish<HD, BF16, 1, TT_ROWS, TT_THREADS>(a, red, rm, rs, min(TT_ROWS, total_rows - row0), row0, b, g, n_new, split, tile);

@@ -6,7 +6,7 @@ import pytest
 
 import esolearn_b200 as E
 from esolearn_b200 import _native as N
-from test_gpu_speculative import IO, check_attention, check_verify, gen, make_cache, noise_of, ref_attention, ref_verify, seen_of
+from test_gpu_speculative import IO, check_attention, check_verify, gen, make_cache, noise_of, parents_of, ref_attention, ref_verify, seen_of
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -37,6 +37,67 @@ def test_chains_over_many_tiles_of_drafted_rows(kv, io, hd, page, ctx):
     check_attention(out, ref_attention(q, cache, [ctx], seen_of(t)), io)
     for _ in range(50):
         assert torch.equal(out, E.tree_attention(q, cache, cl, ctx + t))
+
+
+@pytest.mark.parametrize("kv", ["int8", "bf16", "f32"])
+@pytest.mark.parametrize("bad", [1e3, 1e6, -3.0e38, float("inf"), float("nan")])
+@pytest.mark.parametrize("ctx", [64, 100, 127, 190])
+@pytest.mark.parametrize("rep", [8])
+def test_unseen_rows_beside_the_context_have_no_influence(kv, bad, ctx, rep):
+    # drafted rows that share a tile with context, or begin one: what a token does not see changes no bit of its output,
+    # with rep * 9 query rows per kv head
+    g = gen(ctx)
+    nkv, hd, t, spoilt = 2, 128, 9, 4
+    cache = make_cache(g, 1, 220, nkv, hd, 16, kv)
+    q = torch.randn(1, t, rep * nkv, hd, generator=g, device="cuda") * 0.1
+    parents = parents_of(t, 2)
+    seen = seen_of(t, parents)
+    mask = torch.from_numpy(E.tree_mask(parents)).cuda()
+    cl = ints([ctx])
+    clean = E.tree_attention(q, cache, cl, ctx + t, mask=mask)
+    check_attention(clean, ref_attention(q, cache, [ctx], seen), "f32")
+    for p in [ctx + spoilt] + list(range(ctx + t, 220)):
+        page, slot = int(cache.page_table[0, p // 16]), p % 16
+        for x in ((cache.k_scale, cache.v_scale) if kv == "int8" else (cache.k, cache.v)):
+            x[page, :, slot] = bad
+    out = E.tree_attention(q, cache, cl, ctx + t, mask=mask)
+    blind = ~seen[:, spoilt]
+    assert 0 < int(blind.sum()) < t
+    assert torch.equal(out[:, blind], clean[:, blind])
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("rep", [24])
+@pytest.mark.parametrize("first,count", [(0, 140), (0, 3), (150, 1), (70, 60), (300, 40)])
+@pytest.mark.parametrize("large", [1e3, 1e6, 1e9])
+def test_seen_rows_of_large_scale_and_little_weight(io, rep, first, count, large):
+    # rows of large v_scale that hardly any weight falls on, before, among and behind those that take it all, must not
+    # cost these their bits (3 * rep query rows per kv head)
+    g = gen(first + rep)
+    nkv, hd, t, ctx = 2, 64, 3, 400
+    cache = make_cache(g, 1, ctx + t, nkv, hd, 64, "int8")
+    away = torch.where(torch.rand(hd, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    q = ((away + 0.1 * torch.randn(1, t, rep * nkv, hd, generator=g, device="cuda")) * 0.5).to(IO[io])
+    for p in range(first, first + count):
+        page, slot = int(cache.page_table[0, p // 64]), p % 64
+        cache.k[page, :, slot] = (-100 * away).to(torch.int8)
+        cache.k_scale[page, :, slot] = 0.03  # a score of about -96
+        cache.v_scale[page, :, slot] = large
+    out = E.tree_attention(q, cache, ints([ctx]), ctx + t)
+    check_attention(out, ref_attention(q, cache, [ctx], seen_of(t)), io)
+
+
+@pytest.mark.parametrize("size", [1e-10, 1e-2, 1.0])
+def test_scales_of_any_size_with_many_rows(size):
+    # v_scale over 12 orders of magnitude, zero scales, queries over 20, 72 query rows per kv head
+    g = gen(6)
+    cache = make_cache(g, 1, 400, 2, 64, 64, "int8")
+    cache.v_scale.copy_(10.0 ** (torch.rand(cache.v_scale.shape, generator=g, device="cuda") * 12 - 6))
+    cache.v_scale[:, :, 5] = 0
+    cache.k_scale[:, :, 9] = 0
+    q = torch.randn(1, 9, 16, 64, generator=g, device="cuda") * size * 0.1
+    cl = ints([350])
+    check_attention(E.tree_attention(q, cache, cl, 359), ref_attention(q, cache, [350], seen_of(9)), "f32")
 
 
 # ---------------------------------------------------------------------------
