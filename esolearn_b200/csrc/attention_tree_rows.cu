@@ -397,9 +397,12 @@ __global__ void __launch_bounds__(tr_warps(NR) * 32, 2) tree_attn_rows_kernel(co
                     for (int mt = 0; mt < MT; mt++) x = fmaxf(x, fmaxf(s[mt][nr][e], s[mt][nr][2 + e]));
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                    alpha[nr][e] = m[nr][e] == -INFINITY ? 0.0f : ex2(m[nr][e] - x);
-                    l[nr][e] *= alpha[nr][e];
-                    m[nr][e] = x;
+                    // a row whose own scores are in range keeps its reference, whatever the warp's other rows see
+                    if (x > m[nr][e] + 8.0f) {
+                        alpha[nr][e] = m[nr][e] == -INFINITY ? 0.0f : ex2(m[nr][e] - x);
+                        l[nr][e] *= alpha[nr][e];
+                        m[nr][e] = x;
+                    }
                 }
         }
         bool over = false;

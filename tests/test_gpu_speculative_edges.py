@@ -66,6 +66,13 @@ def test_unseen_rows_beside_the_context_have_no_influence(kv, bad, ctx, rep):
     assert torch.equal(out[:, blind], clean[:, blind])
 
 
+@pytest.mark.parametrize("kv", ["int8", "bf16", "f32"])
+@pytest.mark.parametrize("bad", [1e3, 1e6, -3.0e38, float("inf"), float("nan")])
+@pytest.mark.parametrize("ctx", [64, 100, 127, 190])
+def test_unseen_rows_have_no_influence_on_few_query_rows(kv, bad, ctx):
+    test_unseen_rows_beside_the_context_have_no_influence(kv, bad, ctx, 1)
+
+
 @pytest.mark.parametrize("io", ["f32", "bf16"])
 @pytest.mark.parametrize("rep", [24])
 @pytest.mark.parametrize("first,count", [(0, 140), (0, 3), (150, 1), (70, 60), (300, 40)])
