@@ -399,9 +399,19 @@ __global__ void __launch_bounds__(tr_warps(NR) * 32, 2) tree_attn_rows_kernel(co
                     for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
                     // a row whose own scores are in range keeps its reference, whatever the warp's other rows see
                     if (x > m[nr][e] + 8.0f) {
-                        alpha[nr][e] = m[nr][e] == -INFINITY ? 0.0f : ex2(m[nr][e] - x);
+                        const float down = m[nr][e] - x;  // -inf at first
+                        alpha[nr][e] = ex2(down);
                         l[nr][e] *= alpha[nr][e];
                         m[nr][e] = x;
+                        if (DT == SB_KV_I8 && wlim[nr][e] > 0.0f) {
+                            // the weights so far have shrunk, and the largest of them (kw below) with them: kw rises as far
+                            // (clamped as below), so that a large v_scale which has lost its weight takes no bits from others
+                            const int ex = (int)(__float_as_uint(wlim[nr][e]) >> 23) - 8;
+                            const int lower = min((int)fminf(-down, 256.0f), max(ex - 16, 0));
+                            wlim[nr][e] = __uint_as_float((uint32_t)(ex - lower + 8) << 23);
+                            kw[nr][e] = __uint_as_float((uint32_t)(254 - (ex - lower) + 7) << 23);
+                            alpha[nr][e] = ex2(down + (float)lower);
+                        }
                     }
                 }
         }

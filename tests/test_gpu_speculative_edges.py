@@ -94,6 +94,28 @@ def test_seen_rows_of_large_scale_and_little_weight(io, rep, first, count, large
     check_attention(out, ref_attention(q, cache, [ctx], seen_of(t)), io)
 
 
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("rep", [1, 4, 10])
+@pytest.mark.parametrize("first,count", [(0, 1000), (0, 3), (500, 900)])
+@pytest.mark.parametrize("large", [1e3, 1e6, 1e9])
+def test_seen_rows_of_large_scale_that_later_scores_outweigh(io, rep, first, count, large):
+    # the same with few query rows (3 to 30) and so many sequences that a warp has many tiles: rows of large v_scale that
+    # it meets first, with all the weight there is so far, and that lose it to later ones
+    g = gen(first + rep)
+    b, nkv, hd, t, ctx = 8, 16, 64, 3, 1800
+    cache = make_cache(g, b, ctx + t, nkv, hd, 64, "int8")
+    away = torch.where(torch.rand(hd, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    q = ((away + 0.1 * torch.randn(b, t, rep * nkv, hd, generator=g, device="cuda")) * 0.5).to(IO[io])
+    p = torch.arange(first, first + count, device="cuda")
+    for i in range(b):
+        page, slot = cache.page_table[i].long()[p // 64], p % 64
+        cache.k[page, :, slot] = (-100 * away).to(torch.int8)
+        cache.k_scale[page, :, slot] = 0.03  # a score of about -96
+        cache.v_scale[page, :, slot] = large
+    out = E.tree_attention(q, cache, ints([ctx] * b), ctx + t)
+    check_attention(out, ref_attention(q, cache, [ctx] * b, seen_of(t)), io)
+
+
 @pytest.mark.parametrize("size", [1e-10, 1e-2, 1.0])
 def test_scales_of_any_size_with_many_rows(size):
     # v_scale over 12 orders of magnitude, zero scales, queries over 20, 72 query rows per kv head
