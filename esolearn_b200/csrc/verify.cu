@@ -84,6 +84,8 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Exponents are (x - max) c everywhere, in sums, joins and probabilities: x c - max c in one FMA would round max c, by
+// more than one at low temperatures, and scale the sum against the probabilities.
 // (max, sum of 2^((x - max) c)) of two parts
 __device__ __forceinline__ float2 join_stat(float2 a, float2 b, float c) {
     const float m = fmaxf(a.x, b.x);
@@ -123,9 +125,8 @@ __global__ void __launch_bounds__(ST) verify_stats_kernel(const float *logits, l
 #pragma unroll
     for (int k = 0; k < SE; k++) st.x = fmaxf(st.x, x[k]);
     if (st.x > -INFINITY) {
-        const float off = -st.x * c;
 #pragma unroll
-        for (int k = 0; k < SE; k++) st.y += ex2(fmaf(x[k], c, off));
+        for (int k = 0; k < SE; k++) st.y += ex2((x[k] - st.x) * c);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) st = join_stat(st, make_float2(__shfl_xor_sync(0xffffffffu, st.x, o), __shfl_xor_sync(0xffffffffu, st.y, o)), c);
@@ -346,9 +347,8 @@ __global__ void __launch_bounds__(VT, 1) verify_kernel(const VerifyArgs a, int t
             if (PRE) st = s.pm[node];
             if (!PRE) over_row(node, buf, [&](int, float4 x, auto) { st.x = fmaxf(st.x, fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w))); });
             if (!PRE && st.x > -INFINITY) {
-                const float off = -st.x * c;
                 over_row(node, buf, [&](int, float4 x, auto) {
-                    st.y += (ex2(fmaf(x.x, c, off)) + ex2(fmaf(x.y, c, off))) + (ex2(fmaf(x.z, c, off)) + ex2(fmaf(x.w, c, off)));
+                    st.y += (ex2((x.x - st.x) * c) + ex2((x.y - st.x) * c)) + (ex2((x.z - st.x) * c) + ex2((x.w - st.x) * c));
                 });
             }
             if (!PRE) st = all_stat(st);

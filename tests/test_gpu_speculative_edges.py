@@ -172,3 +172,29 @@ def test_noise_shared_by_the_batch(b, v, draft):
             path, tok, near = ref_verify(logits[i], tokens[i], parents.tolist(), u[i], noise[i], 1.0, None if q is None else q[i])
             if near > 1e-4:
                 assert got[0][i].tolist() == path + [-1] * (3 - len(path)) and int(got[2][i]) == tok
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("b,n,v", [(8, 5, 1000), (40, 9, 128256)])
+@pytest.mark.parametrize("temp,shift", [(1e-2, 0.0), (1e-4, 0.0), (1e-6, 0.0), (0.7, 1e3), (0.7, -1e4), (0.05, 1e3)])
+def test_verify_at_low_temperatures_and_shifted_logits(b, n, v, temp, shift, draft):
+    """Two tokens share each row's probability and thresholds lie within 2e-4 of it, closer than a sum that is scaled
+    against its terms would allow, and farther than rounding (a few 2^-24 of logits that are equal but for the gap)."""
+    g = gen(n + v)
+    logits = torch.randn(b, n, v, generator=g, device="cuda") * 2 + 20 * max(temp, 1.0) + shift
+    top = logits.amax(-1) + 30 * temp
+    pair = torch.stack([torch.randperm(v, generator=g, device="cuda")[:2] for _ in range(b * n)]).view(b, n, 2)
+    # representable gaps of half a temperature or so: what the 64-bit walk sees is what the kernel is given
+    logits.scatter_(2, pair, torch.stack([top, top - 0.5 * temp], -1))
+    parents = torch.arange(-1, n - 1, dtype=torch.int32, device="cuda")
+    p = torch.softmax(logits.double() / temp, -1)
+    tokens = torch.zeros(b, n, dtype=torch.int32, device="cuda")
+    tokens[:, 1:] = pair[:, :-1, 0].int()
+    mine = p[:, :-1].gather(2, pair[:, :-1, :1])[..., 0]
+    q = None
+    if draft:  # the draft has half of that token's probability over again: accepted when u q < p
+        q = torch.zeros(b, n, v, device="cuda").scatter_(2, pair, torch.stack([torch.ones(b, n, device="cuda"), torch.zeros(b, n, device="cuda")], -1))
+    u = torch.rand(b, n, generator=g, device="cuda")
+    near = 1 + 2e-4 * torch.where(torch.rand(b, n - 1, generator=g, device="cuda") < 0.8, -1.0, 1.0)
+    u[:, 1:] = (mine * near).float()
+    check_verify(logits, tokens, parents, u, noise_of(g, b, v), temp, q)
