@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(APPEND_THREADS) kv_append_kernel(const KvAppen
         }
         if (h < nh) {
 #pragma unroll
-            for (int j = 0; j < E; j++) x[j] = turned ? __fmul_rn(x[j], a.q_scale) : 0.0f;
+            for (int j = 0; j < E; j++) x[j] = r0 >= 0 ? __fmul_rn(x[j], a.q_scale) : 0.0f;
             Io<BF16>::store(qo + h * HD, x);
         }
         // the other heads' rows of a warp go on together: a row's maximum is taken over its lanes

@@ -6,7 +6,7 @@ import pytest
 
 import esolearn_b200 as E
 from esolearn_b200 import _native as N
-from test_gpu_speculative import IO, check_attention, check_verify, gen, make_cache, noise_of, parents_of, ref_attention, ref_verify, seen_of
+from test_gpu_speculative import IO, check_attention, check_verify, gen, make_cache, noise_of, parents_of, ref_attention, ref_verify, rope_tables, seen_of
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -127,6 +127,27 @@ def test_scales_of_any_size_with_many_rows(size):
     q = torch.randn(1, 9, 16, 64, generator=g, device="cuda") * size * 0.1
     cl = ints([350])
     check_attention(E.tree_attention(q, cache, cl, 359), ref_attention(q, cache, [350], seen_of(9)), "f32")
+
+
+# ---------------------------------------------------------------------------
+# the cache
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", ["int8", "bf16", "f32"])
+@pytest.mark.parametrize("rope", [False, True])
+def test_q_of_rows_outside_the_cache_is_zero(kv, io, rope):
+    # rows on a page that does not exist, behind the table's end, before its start and behind n_new write nothing
+    g = gen(2)
+    cache = make_cache(g, 5, 32, 2, 64, 16, kv)
+    cache.page_table[0, 1] = 10 ** 6
+    cache.page_table[1, 1] = -1
+    x = (torch.randn(5, 8, 8, 64, generator=g, device="cuda") + 4).to(IO[io])
+    q, k, v = x.split([4, 2, 2], 2)
+    q_out = torch.full((5, 8, 4, 64), 7.0, dtype=IO[io], device="cuda")
+    E.kv_append(cache, k, v, ints([12, 12, 28, -3, 0]), q=q, rope=rope_tables(100, 64) if rope else None, n_new=ints([8, 8, 8, 8, 5]), q_out=q_out)
+    written = [4, 4, 4, 0, 5]
+    for b, n in enumerate(written):
+        assert not q_out[b, n:].any() and bool(q_out[b, :n].any(-1).all())
 
 
 # ---------------------------------------------------------------------------
