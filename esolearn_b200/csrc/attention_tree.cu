@@ -98,6 +98,7 @@ __global__ void __launch_bounds__(TA_THREADS) tree_attn_kernel(const TreeAttnArg
     const int cap = a.c.pg.max_pages * a.c.pg.page_size;
     const int ctx = min(max(a.ctx_len[b], 0), cap);
     const int n_new = a.n_new ? min(max(a.n_new[b], 0), a.T) : a.T;
+    const int n_vis = min(n_new, cap - ctx);  // tokens behind the table have no rows to be seen
     // the last token of this CTA's rows; under the j <= i rule nothing behind it is read
     const int last_i = min((min(row0 + ROWS, total_rows) - 1) / a.rep, n_new - 1);
     const int len = (int)min((long long)cap, (long long)ctx + (a.mask ? n_new : last_i + 1));
@@ -217,8 +218,8 @@ __global__ void __launch_bounds__(TA_THREADS) tree_attn_kernel(const TreeAttnArg
         const bool tail = base + TILE > ctx;
         unsigned long long va = ~0ull, vb = ~0ull;
         if (tail) {
-            va = visible_bits(a, b, ia, ctx, n_new, base) >> (wp * PW);
-            vb = visible_bits(a, b, ib, ctx, n_new, base) >> (wp * PW);
+            va = visible_bits(a, b, ia, ctx, n_vis, base) >> (wp * PW);
+            vb = visible_bits(a, b, ib, ctx, n_vis, base) >> (wp * PW);
         }
         float na = ma, nb = mb;
 #pragma unroll

@@ -94,17 +94,18 @@ __device__ __forceinline__ uint32_t code2_f16(uint32_t w, uint32_t sel) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Bits of positions base .. base+63 that token i sees (bit n: position base + n).
 __device__ __forceinline__ unsigned long long low_bits(long long n) {
     return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
 }
-__device__ __forceinline__ unsigned long long visible_bits(const TreeAttnArgs &a, int b, int i, long long ctx, int n_new,
+// Bits of positions base .. base+63 that token i sees (bit n: position base + n); of the tokens only the first n_vis are
+// there to be seen (the others do not exist, have no place in the table, or lie behind all rows of the CTA).
+__device__ __forceinline__ unsigned long long visible_bits(const TreeAttnArgs &a, int b, int i, long long ctx, int n_vis,
                                                            long long base) {
     const long long j0 = base - ctx;  // token index of bit 0 (negative: context)
     unsigned long long w = low_bits(-j0);
     if (i < 0) return w;
     if (!a.mask) {
-        w |= low_bits((long long)min(i + 1, n_new) - j0);
+        w |= low_bits((long long)min(i + 1, n_vis) - j0);
     } else {
         const unsigned long long *row = a.mask + (size_t)b * a.mask_ld + (size_t)i * a.mask_words;
         unsigned long long m = 0;
@@ -115,7 +116,7 @@ __device__ __forceinline__ unsigned long long visible_bits(const TreeAttnArgs &a
             if (k < a.mask_words) m = __ldg(row + k) >> s;
             if (s && k + 1 < a.mask_words) m |= __ldg(row + k + 1) << (64 - s);
         }
-        w |= m & low_bits((long long)n_new - j0);
+        w |= m & low_bits((long long)n_vis - j0);
     }
     return w;
 }

@@ -158,8 +158,8 @@ __global__ void __launch_bounds__(tr_warps(NR) * 32, 2) tree_attn_rows_kernel(co
 
     const int cap = a.c.pg.max_pages * a.c.pg.page_size;
     const int ctx = min(max(a.ctx_len[b], 0), cap);
-    const int n_new = a.n_new ? min(max(a.n_new[b], 0), a.T) : a.T;
-    const int len = (int)min((long long)cap, (long long)ctx + n_new);
+    auto tokens = [&]() { return a.n_new ? min(max(a.n_new[b], 0), a.T) : a.T; };  // (read where it is needed: a register less)
+    const int len = ctx + min(tokens(), cap - ctx);
     const int ntiles = (len + PW - 1) / PW;
     const int per = (ntiles + a.n_splits - 1) / a.n_splits;
     const int t0 = min(split * per, ntiles) + warp, t1 = min(min(split * per, ntiles) + per, ntiles);
@@ -369,8 +369,8 @@ __global__ void __launch_bounds__(tr_warps(NR) * 32, 2) tree_attn_rows_kernel(co
                 seen[nr][e] = ~0u;
                 if (tail) {
                     const int r = nr * 8 + 2 * c4 + e;
-                    const int i = r < total_rows && r / a.rep < n_new ? r / a.rep : -1;
-                    seen[nr][e] = (unsigned)visible_bits(a, b, i, ctx, n_new, base);
+                    const int i = r < total_rows && r / a.rep < tokens() ? r / a.rep : -1;
+                    seen[nr][e] = (unsigned)visible_bits(a, b, i, ctx, len - ctx, base);
                 }
             }
 #pragma unroll
@@ -611,7 +611,7 @@ __global__ void __launch_bounds__(tr_warps(NR) * 32, 2) tree_attn_rows_kernel(co
         }
     __syncthreads();
     const size_t tile = (size_t)b * nkv + g;
-    tree_finish<HD, BF16, TR_WARPS, ROWS, TR_THREADS>(a, red, rm, rl, min(ROWS, total_rows), 0, b, g, n_new, split, tile);
+    tree_finish<HD, BF16, TR_WARPS, ROWS, TR_THREADS>(a, red, rm, rl, min(ROWS, total_rows), 0, b, g, tokens(), split, tile);
 }
 
 template <int HD, int DT, bool BF16, int NR>

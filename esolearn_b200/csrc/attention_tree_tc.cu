@@ -249,6 +249,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
     const int cap = a.c.pg.max_pages * a.c.pg.page_size;
     const int ctx = min(max(a.ctx_len[b], 0), cap);
     const int n_new = a.n_new ? min(max(a.n_new[b], 0), a.T) : a.T;
+    const int n_vis = min(n_new, cap - ctx);  // tokens behind the table have no rows to be seen
     // the last token of these rows; under the j <= i rule nothing behind it is read
     const int last_i = min((min(row0 + TT_ROWS, total_rows) - 1) / a.rep, n_new - 1);
     const int len = (int)min((long long)cap, (long long)ctx + (a.mask ? n_new : last_i + 1));
@@ -426,7 +427,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
             const int pos0 = (t0 + t) * TT_TILE + half * 64;
             const bool tail = pos0 + 64 > ctx;
             unsigned long long vis = ~0ull;
-            if (tail) vis = visible_bits(a, b, iv, ctx, n_new, pos0);
+            if (tail) vis = visible_bits(a, b, iv, ctx, n_vis, pos0);
             if (DT == SB_KV_I8) wait(sc_full + 8 * (t % TT_SCALES), (t / TT_SCALES) & 1);
             wait(s_full + 8 * sb, (t / C::NSB) & 1);
             tc_fence_after();
@@ -587,7 +588,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
                 // the tile's non-finite V elements (zeros in the product) reach the rows that see them
                 const int p0 = (t0 + t) * TT_TILE;
                 for (int h = 0; h < 2; h++) {
-                    const unsigned long long vis = visible_bits(a, b, iv, ctx, n_new, p0 + h * 64);
+                    const unsigned long long vis = visible_bits(a, b, iv, ctx, n_vis, p0 + h * 64);
                     for (int j = 0; j < 64; j++) {
                         const int p = p0 + h * 64 + j;
                         if (p >= len || !((vis >> j) & 1)) continue;

@@ -192,7 +192,8 @@ sb_status sb_attn_decode_paged_noalloc(const float *q, const void *k_cache, cons
  * page_table: device [B][max_pages] page numbers.  head_dim is 64 or 128.  All
  * pointers 16-byte aligned.  Positions outside the table and page numbers
  * outside 0..n_pages-1 are never accessed: such rows are not written and read
- * as zeros.  The struct is read during the call only. */
+ * as zeros (attention: positions outside the table are seen by no token).  The
+ * struct is read during the call only. */
 typedef struct sb_kv_cache {
     void *k, *v;
     float *k_scale, *v_scale;

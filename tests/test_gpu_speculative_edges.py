@@ -6,7 +6,7 @@ import pytest
 
 import esolearn_b200 as E
 from esolearn_b200 import _native as N
-from test_gpu_speculative import IO, check_attention, check_verify, gen, make_cache, noise_of, parents_of, ref_attention, ref_verify, rope_tables, seen_of
+from test_gpu_speculative import IO, check_attention, check_verify, gen, make_cache, noise_of, parents_of, ref_attention, ref_verify, rope_tables, rows_of, seen_of
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -127,6 +127,29 @@ def test_scales_of_any_size_with_many_rows(size):
     q = torch.randn(1, 9, 16, 64, generator=g, device="cuda") * size * 0.1
     cl = ints([350])
     check_attention(E.tree_attention(q, cache, cl, 359), ref_attention(q, cache, [350], seen_of(9)), "f32")
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", ["int8", "bf16", "f32"])
+@pytest.mark.parametrize("page,max_pages", [(8, 5), (7, 6), (48, 1), (16, 8), (64, 3)])
+@pytest.mark.parametrize("rep", [1, 12])
+def test_positions_behind_the_table_are_seen_by_no_token(kv, io, page, max_pages, rep):
+    # more tokens than the table has room for (one sequence by five, one full before the call): what has no place in the
+    # cache is not there, for tokens inside and outside alike, whatever shared memory held before the call
+    g = gen(page + rep)
+    cap, t, nkv, hd = page * max_pages, 9, 2, 64
+    cache = make_cache(g, 2, cap, nkv, hd, page, kv)
+    q = (torch.randn(2, t, rep * nkv, hd, generator=g, device="cuda") * 0.2).to(IO[io])
+    ctx = [cap - 4, cap]
+    parents = parents_of(t, 2)
+    for mask, seen in ((None, seen_of(t)), (torch.from_numpy(E.tree_mask(parents)).cuda(), seen_of(t, parents))):
+        out = E.tree_attention(q, cache, ints(ctx), cap + t, mask=mask)
+        for b in range(2):
+            k, v = (rows_of(cache, x, b, cap) for x in ("k", "v"))
+            sees = torch.cat([torch.ones(t, ctx[b], dtype=torch.bool, device="cuda"), seen[:, :cap - ctx[b]]], 1)
+            x = torch.einsum("tgrd,ngd->tgrn", q[b].double().view(t, nkv, rep, hd), k).masked_fill(~sees[:, None, None], -float("inf"))
+            ref = torch.einsum("tgrn,ngd->tgrd", torch.softmax(x, -1), v).reshape(1, t, rep * nkv, hd)
+            check_attention(out[b:b + 1], ref, io)
 
 
 # ---------------------------------------------------------------------------
