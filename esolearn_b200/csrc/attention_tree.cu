@@ -18,7 +18,7 @@
 // The products run on the tensor cores and keep f32's accuracy by splitting
 // the f32 operand into a sum of terms of the other's type:
 //   bf16 cache: q and p as three bf16 terms (2^-26), two for p when q and out
-//     are bf16 (tcgen05 kernel: two for p in any case);
+//     are bf16 (2^-18, against the output's 2^-9);
 //   int8 cache: codes are exact in f16; q (over a power of two of its row's
 //     magnitude) and p * v_scale (over a power of two of its row's) as two
 //     f16 terms (2^-22); k_scale multiplies the scores;

@@ -9,8 +9,8 @@
 //     magnitude) as two f16 terms (one when q is bf16); k_scale multiplies the
 //     scores; p * v_scale, over a power of two of the largest that the row sees,
 //     as two f16 terms;
-//   bf16 cache: K and V as they are, q as three bf16 terms (one when q is
-//     bf16), p as two.
+//   bf16 cache: K and V as they are, q and p as three bf16 terms (one and two
+//     when q is bf16).
 // Each tile's O starts from zero and is added to the row's sums in registers in
 // f32: the tensor cores truncate as they accumulate.
 //
@@ -26,8 +26,9 @@
 //     the scales; bf16: TMA boxes (pages of a multiple of eight positions).
 //   warp 15: one thread issues the products: q K^T of tile t before p V of tile
 //     t-1, so the first runs under the softmax of t-1.
-// TMEM: three score tiles (p over them) and O; or two, q and O, where shared
-// memory has no room for q (int8 cache, f32 q, head_dim 128).
+// TMEM: three score tiles (p over them) and O; two where p has three terms (bf16
+// cache, f32 q); two, q and O where shared memory has no room for q (int8 cache,
+// f32 q, head_dim 128).
 //
 // Shared-memory operands use the 128-byte swizzle: rows of 64 16-bit elements
 // (128 bytes, of 128 rows; head_dim 128 is two such blocks), piece c of row r
@@ -74,10 +75,14 @@ constexpr float TT_KW = 7.0f, TT_KW_MAX = 14.0f;
 
 template <int HD, int DT, bool BF16>
 struct TtShape {
+    // terms of q and of p: f32's accuracy with an f32 q (bf16 terms hold 8 bits each, f16 terms 11); where q and the output
+    // are bf16, p's two bf16 terms leave 2^-18, well below the output's rounding
     static constexpr int QT = BF16 ? 1 : DT == SB_KV_BF16 ? 3 : 2;
-    // q in TMEM where shared memory has no room for it; TMEM then has room for two score tiles instead of three
+    static constexpr int PT = DT == SB_KV_BF16 && !BF16 ? 3 : 2;
+    // q in TMEM where shared memory has no room for it; TMEM then has room for two score tiles instead of three, as it has where p has three terms
     static constexpr bool QTMEM = DT == SB_KV_I8 && !BF16 && HD == 128;
-    static constexpr int NSB = QTMEM ? 2 : 3;
+    static constexpr int NSB = QTMEM || PT == 3 ? 2 : 3;
+    static constexpr int T_S = PT * 64;             // TMEM columns of a score tile, 128, and of p's terms, which take its place
     static constexpr int NS = 2;                    // stages of K and of V
     static constexpr int T_Q = 256, T_O = 384;      // TMEM columns; scores from 0
     static constexpr int MAT = 128 * HD * 2;        // bytes of a 128-row 16-bit tile
@@ -93,6 +98,7 @@ struct TtShape {
     static constexpr int BAR_OFF = AL_OFF + 4 * 128;
     static constexpr int BYTES = BAR_OFF + 448;
     static constexpr int JOIN = 128 * (HD + 2) * 4;  // the row sums at the end, over the stages and q
+    static_assert(NSB * T_S <= (QTMEM ? T_Q : T_O), "TMEM columns");
     static_assert(JOIN <= SC_OFF, "the row sums must fit the tiles");
     static_assert(RAWK % 128 == 0 && RAWV % 128 == 0, "bulk copies");
 };
@@ -174,27 +180,23 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// (x, y) as two pairs of 16-bit terms
-template <int DT>
-__device__ __forceinline__ void split2(uint64_t v, uint32_t &hi, uint32_t &lo) {
-    const float2 x = unpack2(v);
-    float2 h;
-    if (DT == SB_KV_I8) {
-        const __half2 p = __floats2half2_rn(x.x, x.y);
-        hi = *reinterpret_cast<const uint32_t *>(&p);
-        h = __half22float2(p);
-    } else {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(x.x, x.y);
-        hi = *reinterpret_cast<const uint32_t *>(&p);
-        h = make_float2(__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u));
-    }
-    const float2 d = unpack2(fma2(pack2(h.x, h.y), pack2(-1.0f, -1.0f), v));
-    if (DT == SB_KV_I8) {
-        const __half2 p = __floats2half2_rn(d.x, d.y);
-        lo = *reinterpret_cast<const uint32_t *>(&p);
-    } else {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(d.x, d.y);
-        lo = *reinterpret_cast<const uint32_t *>(&p);
+// (x, y) as TERMS pairs of 16-bit terms
+template <int DT, int TERMS>
+__device__ __forceinline__ void split2(uint64_t v, uint32_t (&o)[TERMS]) {
+#pragma unroll
+    for (int t = 0; t < TERMS; t++) {
+        const float2 x = unpack2(v);
+        float2 h;
+        if (DT == SB_KV_I8) {
+            const __half2 p = __floats2half2_rn(x.x, x.y);
+            o[t] = *reinterpret_cast<const uint32_t *>(&p);
+            h = __half22float2(p);
+        } else {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(x.x, x.y);
+            o[t] = *reinterpret_cast<const uint32_t *>(&p);
+            h = make_float2(__uint_as_float(o[t] << 16), __uint_as_float(o[t] & 0xffff0000u));
+        }
+        if (t + 1 < TERMS) v = fma2(pack2(h.x, h.y), pack2(-1.0f, -1.0f), v);
     }
 }
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
@@ -423,7 +425,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
         for (int t = 0; t < nt; t++) {
             const int buf = t & 1;
             const int sb = t % C::NSB;
-            const uint32_t S = tmem + lanes + sb * 128;
+            const uint32_t S = tmem + lanes + sb * C::T_S;
             const int pos0 = (t0 + t) * TT_TILE + half * 64;
             const bool tail = pos0 + 64 > ctx;
             unsigned long long vis = ~0ull;
@@ -509,7 +511,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
             auto weights = [&](auto masked) {
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    uint32_t hi[8], lo[8];
+                    uint32_t term[C::PT][8];
 #pragma unroll
                     for (int j = 0; j < 8; j++) {
                         const float2 x = unpack2(fma2(s[c * 8 + j], f2, off2));
@@ -524,10 +526,13 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
                                 p = pack2(w.x, w.y);
                             }
                         }
-                        split2<DT>(p, hi[j], lo[j]);
+                        uint32_t u[C::PT];
+                        split2<DT>(p, u);
+#pragma unroll
+                        for (int q = 0; q < C::PT; q++) term[q][j] = u[q];
                     }
-                    tmem_st8(S + half * 32 + c * 8, hi);
-                    tmem_st8(S + 64 + half * 32 + c * 8, lo);
+#pragma unroll
+                    for (int q = 0; q < C::PT; q++) tmem_st8(S + q * 64 + half * 32 + c * 8, term[q]);
                 }
             };
             if (DT == SB_KV_I8 && tail) weights(std::true_type{});
@@ -795,8 +800,8 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
 #pragma unroll
                     for (int k = 0; k < HD / 16; k++) {
                         const int at = (k >> 2) * (16384 >> 4) + (k & 3) * 2;  // 64 elements a block, 32 bytes a step
-                        if (C::QTMEM) umma_ts(tmem + buf * 128, tmem + C::T_Q + q * (HD / 2) + k * 8, kd + at, id_s, q != QT - 1 || k > 0);
-                        else umma_ss(tmem + buf * 128, qd + at, kd + at, id_s, q != QT - 1 || k > 0);
+                        if (C::QTMEM) umma_ts(tmem + buf * C::T_S, tmem + C::T_Q + q * (HD / 2) + k * 8, kd + at, id_s, q != QT - 1 || k > 0);
+                        else umma_ss(tmem + buf * C::T_S, qd + at, kd + at, id_s, q != QT - 1 || k > 0);
                         pace((QT - 1 - q) * (HD / 16) + k);
                     }
                 }
@@ -810,11 +815,11 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
                 pace_from = clock32();
                 const uint64_t vd = sw128_desc(base + stage * C::STAGE, 16384);
 #pragma unroll
-                for (int q = 1; q >= 0; q--)
+                for (int q = C::PT - 1; q >= 0; q--)
 #pragma unroll
                     for (int k = 0; k < TT_TILE / 16; k++) {
-                        umma_ts(tmem + C::T_O, tmem + buf * 128 + q * 64 + k * 8, vd + k * (2048 >> 4), id_o, q != 1 || k > 0);
-                        pace((1 - q) * (TT_TILE / 16) + k);
+                        umma_ts(tmem + C::T_O, tmem + buf * C::T_S + q * 64 + k * 8, vd + k * (2048 >> 4), id_o, q != C::PT - 1 || k > 0);
+                        pace((C::PT - 1 - q) * (TT_TILE / 16) + k);
                     }
                 umma_commit(pv_done + 8 * buf);
             }

@@ -6,7 +6,7 @@ import pytest
 
 import esolearn_b200 as E
 from esolearn_b200 import _native as N
-from test_gpu_speculative import IO, check_attention, check_verify, gen, make_cache, noise_of, parents_of, ref_attention, ref_verify, rope_tables, rows_of, seen_of
+from test_gpu_speculative import IO, check_attention, check_verify, gen, make_cache, noise_of, parents_of, ref_attention, ref_verify, rope_tables, rows_of, seen_of, words
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -37,6 +37,24 @@ def test_chains_over_many_tiles_of_drafted_rows(kv, io, hd, page, ctx):
     check_attention(out, ref_attention(q, cache, [ctx], seen_of(t)), io)
     for _ in range(50):
         assert torch.equal(out, E.tree_attention(q, cache, cl, ctx + t))
+
+
+@pytest.mark.parametrize("kv", ["int8", "bf16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("rep,t", [(1, 5), (4, 7), (3, 40), (1, 200)])
+def test_a_single_seen_row_is_returned_to_f32_accuracy(kv, hd, rep, t):
+    # no context, and each token sees its own row alone: the output is that row of V.  Its weight is 22 bits or more in
+    # terms, each of up to six products of terms is summed in f32 with truncation (2^-23), and 1 / l, the scale and their
+    # products round (2^-24 each): 4 * 2^-22 of the value in all.
+    g = gen(t)
+    nkv = 2
+    cache = make_cache(g, 2, t, nkv, hd, 16, kv)
+    q = torch.randn(2, t, rep * nkv, hd, generator=g, device="cuda") * 2 * hd ** -0.5
+    mask = words(torch.eye(t, dtype=torch.bool))
+    out = E.tree_attention(q, cache, ints([0, 0]), t, mask=mask)
+    for b in range(2):
+        want = rows_of(cache, "v", b, t).repeat_interleave(rep, 1)
+        assert float(((out[b].double() - want).abs() / want.abs().clamp(min=1e-30)).max()) < 2.0 ** -20
 
 
 @pytest.mark.parametrize("kv", ["int8", "bf16", "f32"])
