@@ -146,6 +146,37 @@ static int stream_workspace(size_t bytes, void **out, cudaStream_t st) {
     return SB_OK;
 }
 
+// The words of wait_errors.cuh.  (Allocating them is no work of any stream: a
+// capture that the thread's stream is in does not mind.)
+static unsigned *g_wait_errors = nullptr;
+static std::mutex g_wait_errors_mu;
+
+int wait_error_words(unsigned **words) {
+    std::lock_guard<std::mutex> lock(g_wait_errors_mu);
+    if (!g_wait_errors) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        SB_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
+        void *p = nullptr;
+        const cudaError_t rc = cudaHostAlloc(&p, WAIT_ERRORS * sizeof(unsigned), cudaHostAllocPortable | cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (rc != cudaSuccess) {
+            cudaGetLastError();
+            return set_error(SB_ERR_OOM, "cudaHostAlloc: %s", cudaGetErrorString(rc));
+        }
+        memset(p, 0, WAIT_ERRORS * sizeof(unsigned));
+        g_wait_errors = static_cast<unsigned *>(p);
+    }
+    *words = g_wait_errors;  // unified addressing: devices use the host's address
+    return SB_OK;
+}
+
+int wait_error_check() {
+    std::lock_guard<std::mutex> lock(g_wait_errors_mu);
+    const int e = g_wait_errors ? take_wait_error(g_wait_errors) : -1;
+    SB_CHECK(e < 0, SB_ERR_TIMEOUT, "%s: a bounded wait timed out", e == WAIT_VERIFY ? "draft verification" : "tree attention");
+    return SB_OK;
+}
+
 static int kv_cache_args(const sb_kv_cache *c, const char *who, KvCacheArgs *o) {
     SB_CHECK(c && c->k && c->v && c->page_table, SB_ERR_ARG, "%s: null cache pointer", who);
     SB_CHECK(c->kv_dtype == SB_KV_BF16 || c->kv_dtype == SB_KV_F32 || c->kv_dtype == SB_KV_I8, SB_ERR_ARG,
@@ -258,8 +289,7 @@ sb_status sb_memcpy_d2h(void *dst, const void *src, size_t bytes, void *stream) 
 
 sb_status sb_stream_sync(void *stream) {
     SB_CUDA_TRY(cudaStreamSynchronize((cudaStream_t)stream));
-    SB_TRY(tree_attn_check_error());
-    SB_TRY(verify_check_error());
+    SB_TRY(wait_error_check());
     return qgemv_check_error();
 }
 
@@ -739,6 +769,7 @@ sb_status sb_tree_attention(const sb_kv_cache *cache, const void *q, int dtype, 
     a.ctx_len = ctx_len, a.n_new = n_new;
     a.mask = reinterpret_cast<const unsigned long long *>(mask), a.mask_ld = mask_ld, a.mask_words = words;
     a.out = out;
+    SB_TRY(wait_error_words(&a.errors));
     const int cap = cache->max_pages * cache->page_size;
     const TreeAttnPlan p = tree_attn_plan(a, std::min(std::max(max_ctx, 1), cap));
     a.n_splits = p.n_splits;
@@ -773,6 +804,7 @@ sb_status sb_verify_drafts(const float *logits, int64_t logits_ld, const int32_t
     a.u = u, a.noise = noise, a.ld_noise = noise_ld;
     a.B = B, a.N = N, a.V = V, a.temperature = temperature;
     a.path = path, a.n_accept = n_accept, a.next = next;
+    SB_TRY(wait_error_words(&a.errors));
     void *ws = nullptr;
     if (verify_all_rows(a))
         SB_TRY(stream_workspace(sizeof(float2) * (size_t)B * N * verify_chunks(a), &ws, (cudaStream_t)stream));

@@ -53,8 +53,6 @@ constexpr int TA_THREADS = 128;
 
 constexpr int TA_TILE = 32, TA_STAGES = 2;
 
-__device__ unsigned ta_error_flag = 0;
-
 template <int HD>
 constexpr int ta_pitch() {
     return HD == 128 ? 528 : 272;  // of a row, bytes
@@ -335,7 +333,7 @@ __global__ void __launch_bounds__(TA_THREADS) tree_attn_kernel(const TreeAttnArg
             }
         }
     }
-    if (!ok) atomicExch(&ta_error_flag, 1u);
+    if (!ok) wait_failed(a.errors, WAIT_TREE_F32);
     __syncthreads();
 
     // ---- whole sums of l; O in units of exp(-m)
@@ -494,17 +492,6 @@ int tree_splits(long long base, int tiles, int resident) {
         if (c < cost * 0.999) cost = c, best = s;
     }
     return best;
-}
-
-int tree_attn_f32_check_error() {
-    unsigned f = 0;
-    SB_CUDA_TRY(cudaMemcpyFromSymbol(&f, ta_error_flag, sizeof f));
-    if (f) {
-        const unsigned zero = 0;
-        cudaMemcpyToSymbol(ta_error_flag, &zero, sizeof zero);
-        return set_error(SB_ERR_TIMEOUT, "tree attention: a bounded wait timed out");
-    }
-    return SB_OK;
 }
 
 int tree_attn_launch(const TreeAttnArgs &a, const TreeAttnPlan &p, cudaStream_t st) {

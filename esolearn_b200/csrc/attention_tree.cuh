@@ -5,6 +5,7 @@
 #include <cuda.h>  // CUtensorMap (types only; the encoder is resolved at run time)
 
 #include "kv_cache.cuh"
+#include "wait_errors.cuh"
 
 namespace sb {
 
@@ -30,6 +31,7 @@ struct TreeAttnArgs {
     // box_rows 0: rows are copied one by one.
     int box_rows = 0;
     CUtensorMap tmk, tmv;
+    unsigned *errors = nullptr;  // wait_errors.cuh
 };
 
 // How a call divides its work: rows of one kv head per CTA, tiles of them, and
@@ -48,14 +50,10 @@ int tree_tensor_maps(TreeAttnArgs &a, int max_rows);
 bool tree_attn_rows_wanted(const TreeAttnArgs &a);
 TreeAttnPlan tree_attn_rows_plan(const TreeAttnArgs &a, int max_len);
 int tree_attn_rows_launch(const TreeAttnArgs &a, cudaStream_t st);
-int tree_attn_rows_check_error();
-int tree_attn_f32_check_error();
 // Many rows per kv head over a bf16 or int8 cache (attention_tree_tc.cu).
 bool tree_attn_tc_wanted(const TreeAttnArgs &a);
 TreeAttnPlan tree_attn_tc_plan(const TreeAttnArgs &a, int max_len);
 int tree_attn_tc_launch(const TreeAttnArgs &a, const TreeAttnPlan &p, cudaStream_t st);
-// Reports (and clears) a timed-out wait of any of the kernels.
-int tree_attn_check_error();
 int tree_attn_launch(const TreeAttnArgs &a, const TreeAttnPlan &p, cudaStream_t st);
 
 }  // namespace sb

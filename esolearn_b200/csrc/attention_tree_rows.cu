@@ -65,8 +65,6 @@ struct TrCache {
     static constexpr int SCALES = DT == SB_KV_I8 ? 2 * PW * 4 : 0;
 };
 
-__device__ unsigned tr_error_flag = 0;
-
 // byte offset of chunk `col` of row `row` of a tile of PW rows
 template <int RB, int PW>
 __device__ __forceinline__ int tr_at(int row, int col) {
@@ -588,7 +586,7 @@ __global__ void __launch_bounds__(tr_warps(NR) * 32, 2) tree_attn_rows_kernel(co
         __syncwarp();
     }
     cp_wait<0>();
-    if (!ok && lane == 0) atomicExch(&tr_error_flag, 1u);
+    if (!ok && lane == 0) wait_failed(a.errors, WAIT_TREE_ROWS);
     __syncthreads();
 
     // ---- O in units of exp(-m), whole sums; the warps' shares, then the splits, joined in order
@@ -657,17 +655,6 @@ int tree_attn_rows_launch(const TreeAttnArgs &in, cudaStream_t st) {
     TreeAttnArgs a = in;
     SB_TRY(tree_tensor_maps(a, a.c.dtype == SB_KV_I8 ? 32 : 16));
     return a.c.hd == 128 ? tr_dt<128>(a, st) : tr_dt<64>(a, st);
-}
-
-int tree_attn_rows_check_error() {
-    unsigned f = 0;
-    SB_CUDA_TRY(cudaMemcpyFromSymbol(&f, tr_error_flag, sizeof f));
-    if (f) {
-        const unsigned zero = 0;
-        cudaMemcpyToSymbol(tr_error_flag, &zero, sizeof zero);
-        return set_error(SB_ERR_TIMEOUT, "tree attention: a bounded wait timed out");
-    }
-    return SB_OK;
 }
 
 }  // namespace sb

@@ -55,8 +55,6 @@
 
 namespace sb {
 
-__device__ unsigned tree_attn_error_flag = 0;
-
 namespace {
 
 constexpr int TT_THREADS = 512, TT_ROWS = 128, TT_TILE = 128;
@@ -827,7 +825,7 @@ __global__ void __launch_bounds__(TT_THREADS, 1) tree_attn_tc_kernel(const __gri
         if (ok && nt > 0) ok = mbar_wait_long(pv_done + 8 * ((nt - 1) % C::NSB), ((nt - 1) / C::NSB) & 1);
         }
     }
-    if (!ok) atomicExch(&tree_attn_error_flag, 1u);
+    if (!ok) wait_failed(a.errors, WAIT_TREE_TC);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -863,19 +861,6 @@ int tt_dt(const TreeAttnArgs &a, const TreeAttnPlan &p, cudaStream_t st) {
 }
 
 }  // namespace
-
-int tree_attn_check_error() {
-    SB_TRY(tree_attn_rows_check_error());
-    SB_TRY(tree_attn_f32_check_error());
-    unsigned f = 0;
-    SB_CUDA_TRY(cudaMemcpyFromSymbol(&f, tree_attn_error_flag, sizeof f));
-    if (f) {
-        const unsigned zero = 0;
-        cudaMemcpyToSymbol(tree_attn_error_flag, &zero, sizeof zero);
-        return set_error(SB_ERR_TIMEOUT, "tree attention: a bounded pipeline wait timed out");
-    }
-    return SB_OK;
-}
 
 bool tree_attn_tc_wanted(const TreeAttnArgs &a) { return a.c.dtype != SB_KV_F32 && a.T * a.rep > 32; }
 

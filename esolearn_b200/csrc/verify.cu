@@ -42,8 +42,6 @@
 
 namespace sb {
 
-__device__ unsigned verify_error_flag = 0;
-
 namespace {
 
 namespace cg = cooperative_groups;
@@ -186,7 +184,7 @@ __global__ void __launch_bounds__(VT, 1) verify_kernel(const VerifyArgs a, int t
         const float *src = rows + (size_t)n * a.ld;
         for (int v = bulk + tid; v < len4; v += VT) dst[v] = v < len ? src[v] : -INFINITY;
         if (bulk > 0) {
-            if (!mbar_wait(smem_u32(&bars[buf]), phase[buf])) atomicExch(&verify_error_flag, 1u);
+            if (!mbar_wait(smem_u32(&bars[buf]), phase[buf])) wait_failed(a.errors, WAIT_VERIFY);
             phase[buf] ^= 1;
         }
         __syncthreads();
@@ -426,7 +424,7 @@ __global__ void __launch_bounds__(VT, 1) verify_kernel(const VerifyArgs a, int t
         __syncthreads();  // the row, lx, qx and the list are free again
         if (ahead && (go < 0 || go != child)) {
             // a row that was not needed after all: its copy has to land before its buffer or the CTA goes
-            if (bulk > 0 && !mbar_wait(smem_u32(&bars[buf ^ 1]), phase[buf ^ 1])) atomicExch(&verify_error_flag, 1u);
+            if (bulk > 0 && !mbar_wait(smem_u32(&bars[buf ^ 1]), phase[buf ^ 1])) wait_failed(a.errors, WAIT_VERIFY);
             phase[buf ^ 1] ^= 1;
         }
         if (go < 0) {
@@ -450,17 +448,6 @@ __global__ void __launch_bounds__(VT, 1) verify_kernel(const VerifyArgs a, int t
 }
 
 }  // namespace
-
-int verify_check_error() {
-    unsigned f = 0;
-    SB_CUDA_TRY(cudaMemcpyFromSymbol(&f, verify_error_flag, sizeof f));
-    if (f) {
-        const unsigned zero = 0;
-        cudaMemcpyToSymbol(verify_error_flag, &zero, sizeof zero);
-        return set_error(SB_ERR_TIMEOUT, "verification: a bounded wait timed out");
-    }
-    return SB_OK;
-}
 
 // Rows of all nodes first: where reading them all takes less than the walk's
 // steps, of about 4 us each (all rows of 1e8 bytes take 30 us).  With the draft's

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "sb_common.cuh"
+#include "wait_errors.cuh"
 
 namespace sb {
 
@@ -22,9 +23,8 @@ struct VerifyArgs {
     int *path = nullptr;      // [B][N], -1 behind the accepted nodes
     int *n_accept = nullptr;  // [B]
     int *next = nullptr;      // [B]
+    unsigned *errors = nullptr;  // wait_errors.cuh
 };
-// Reports (and clears) a timed-out wait.
-int verify_check_error();
 // Whether every node's row is read before the walk; `part` then holds
 // B * N * verify_chunks pairs, else it is null.
 bool verify_all_rows(const VerifyArgs &a);

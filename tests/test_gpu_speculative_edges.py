@@ -2,6 +2,11 @@
 
 The references, the tolerances of the attention tests and their derivation are those of test_gpu_speculative.
 """
+import ctypes as C
+import subprocess
+import sys
+import time
+
 import pytest
 
 import esolearn_b200 as E
@@ -260,3 +265,45 @@ def test_verify_at_low_temperatures_and_shifted_logits(b, n, v, temp, shift, dra
     near = 1 + 2e-4 * torch.where(torch.rand(b, n - 1, generator=g, device="cuda") < 0.8, -1.0, 1.0)
     u[:, 1:] = (mine * near).float()
     check_verify(logits, tokens, parents, u, noise_of(g, b, v), temp, q)
+
+
+# ---------------------------------------------------------------------------
+# errors of kernels
+
+def test_a_stream_sync_costs_about_one_blocking_copy():
+    # sb_stream_sync looks at the words that kernels record errors in; on an idle stream that is one small copy (a word
+    # of the int8 linears), not one for each kernel
+    lib = N.lib()
+    word, host = torch.zeros(1, dtype=torch.int32, device="cuda"), C.c_int32()
+
+    def best(f):
+        times = []
+        for _ in range(300):
+            t = time.perf_counter()
+            f()
+            times.append(time.perf_counter() - t)
+        return min(times)
+
+    N.check(lib.sb_stream_sync(None))
+    copy = best(lambda: lib.sb_memcpy_d2h(C.addressof(host), word.data_ptr(), 4, None))
+    assert best(lambda: lib.sb_stream_sync(None)) < 2.5 * copy
+
+
+def test_first_calls_inside_a_capture():
+    # a process whose first call of an operator without a workspace is captured
+    code = """
+import torch, esolearn_b200 as E
+cache = E.KvCache.zeros(1, 16, 1, 64, page_size=16, dtype="bf16")
+cache.v.fill_(3.0)
+q = torch.zeros(1, 1, 1, 64, device="cuda")
+cl = torch.full((1,), 5, dtype=torch.int32, device="cuda")
+out = torch.zeros_like(q)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    E.tree_attention(q, cache, cl, 6, out=out)
+g.replay()
+torch.cuda.synchronize()
+assert bool((out == 3.0).all()), out
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)

@@ -63,3 +63,19 @@ def test_tensors_of_another_device_are_refused(monkeypatch):
     for other in (0, 2):
         with pytest.raises(N.SbError, match=f"cuda:{other}"):
             S._stream(_On(other))
+
+
+def test_recorded_wait_errors_are_taken_one_by_one(tmp_path):
+    """The words that kernels set when a wait gives up: each is reported once and cleared."""
+    src, lib = tmp_path / "w.cpp", tmp_path / "libw.so"
+    src.write_text('#include "wait_errors.cuh"\nextern "C" int take(unsigned *w) { return sb::take_wait_error(w); }\n'
+                   'extern "C" int words() { return sb::WAIT_ERRORS; }\n')
+    subprocess.run(["g++", "-std=c++17", "-shared", "-fPIC", "-I" + CSRC, "-o", str(lib), str(src)], check=True)
+    l = C.CDLL(str(lib))
+    n = l.words()
+    w = (C.c_uint * n)()
+    assert l.take(w) == -1
+    for i in range(n):
+        w[i] = 1
+    assert [l.take(w) for _ in range(n + 1)] == list(range(n)) + [-1]
+    assert list(w) == [0] * n
