@@ -173,7 +173,8 @@ int wait_error_words(unsigned **words) {
 int wait_error_check() {
     std::lock_guard<std::mutex> lock(g_wait_errors_mu);
     const int e = g_wait_errors ? take_wait_error(g_wait_errors) : -1;
-    SB_CHECK(e < 0, SB_ERR_TIMEOUT, "%s: a bounded wait timed out", e == WAIT_VERIFY ? "draft verification" : "tree attention");
+    SB_CHECK(e < 0, SB_ERR_TIMEOUT, "%s: a bounded wait of an earlier call timed out, its outputs are not valid",
+             e == WAIT_VERIFY ? "draft verification" : "tree attention");
     return SB_OK;
 }
 
@@ -693,6 +694,7 @@ sb_status sb_kv_append(const sb_kv_cache *cache, const void *q, const void *k, c
                        const int32_t *ctx_len, const int32_t *n_new, const int32_t *depth, int depth_ld,
                        const float *rope_cos, const float *rope_sin, int rope_len, float q_scale, void *q_out,
                        void *stream) {
+    SB_TRY(wait_error_check());
     KvAppendArgs a;
     SB_TRY(kv_cache_args(cache, "sb_kv_append", &a.c));
     SB_CHECK((k && v && ctx_len) || B == 0 || T == 0, SB_ERR_ARG, "sb_kv_append: null argument");
@@ -724,6 +726,7 @@ sb_status sb_kv_append(const sb_kv_cache *cache, const void *q, const void *k, c
 
 sb_status sb_kv_commit(const sb_kv_cache *cache, int B, const int32_t *ctx_len, const int32_t *path, int path_ld,
                        const int32_t *n_accept, void *stream) {
+    SB_TRY(wait_error_check());
     KvCacheArgs c;
     SB_TRY(kv_cache_args(cache, "sb_kv_commit", &c));
     SB_CHECK((ctx_len && path && n_accept) || B == 0 || path_ld == 0, SB_ERR_ARG, "sb_kv_commit: null argument");
@@ -734,6 +737,7 @@ sb_status sb_kv_commit(const sb_kv_cache *cache, int B, const int32_t *ctx_len, 
 
 sb_status sb_kv_read(const sb_kv_cache *cache, int B, const int32_t *start, int n, int dtype, void *k_out,
                      void *v_out, void *stream) {
+    SB_TRY(wait_error_check());
     KvCacheArgs c;
     SB_TRY(kv_cache_args(cache, "sb_kv_read", &c));
     SB_CHECK((k_out && v_out) || n == 0 || B == 0, SB_ERR_ARG, "sb_kv_read: null argument");
@@ -747,6 +751,7 @@ sb_status sb_kv_read(const sb_kv_cache *cache, int B, const int32_t *start, int 
 sb_status sb_tree_attention(const sb_kv_cache *cache, const void *q, int dtype, int64_t q_stride, int B, int T,
                             int n_heads, const int32_t *ctx_len, const int32_t *n_new, const uint64_t *mask,
                             int64_t mask_ld, int max_ctx, void *out, void *stream) {
+    SB_TRY(wait_error_check());
     TreeAttnArgs a;
     SB_TRY(kv_cache_args(cache, "sb_tree_attention", &a.c));
     SB_CHECK((q && out && ctx_len) || B == 0 || T == 0, SB_ERR_ARG, "sb_tree_attention: null argument");
@@ -787,6 +792,7 @@ sb_status sb_verify_drafts(const float *logits, int64_t logits_ld, const int32_t
                            int parents_ld, const float *draft_probs, int64_t draft_ld, const float *u,
                            const float *noise, int64_t noise_ld, int B, int N, int V, float temperature,
                            int32_t *path, int32_t *n_accept, int32_t *next, void *stream) {
+    SB_TRY(wait_error_check());
     SB_CHECK(!std::isnan(temperature), SB_ERR_ARG, "sb_verify_drafts: temperature is NaN");
     SB_CHECK(B >= 0 && N >= 1 && N <= VERIFY_MAX_NODES && V >= 1, SB_ERR_SHAPE, "sb_verify_drafts: B %d, N %d, V %d", B, N, V);
     if (B == 0) return SB_OK;

@@ -10,7 +10,8 @@ token, nodes 1..N-1 are drafted, node i under node parents[i] < i.
     ctx_len += n_accept                                               # `token` is the next step's node 0
 
 N = 1 is plain decoding.  The calls run on torch's current stream and wait for
-nothing; their tensors lie on the thread's current device.  Every call goes to
+nothing; their tensors lie on the thread's current device.  A kernel whose wait
+gave up makes a later call raise SbError (SB_ERR_TIMEOUT).  Every call goes to
 libscryb200.so (declarations and the exact rules in include/sb_api.h).  The
 reference decodes one token per step from an f32 cache and has no counterpart.
 """

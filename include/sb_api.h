@@ -193,7 +193,11 @@ sb_status sb_attn_decode_paged_noalloc(const float *q, const void *k_cache, cons
  * pointers 16-byte aligned.  Positions outside the table and page numbers
  * outside 0..n_pages-1 are never accessed: such rows are not written and read
  * as zeros (attention: positions outside the table are seen by no token).  The
- * struct is read during the call only. */
+ * struct is read during the call only.
+ *
+ * Waits inside these kernels are bounded (2 s).  One that gives up leaves the
+ * call's outputs invalid; sb_stream_sync reports it as SB_ERR_TIMEOUT, and where
+ * it is not called the next of these entry points does, in place of its work. */
 typedef struct sb_kv_cache {
     void *k, *v;
     float *k_scale, *v_scale;

@@ -79,3 +79,29 @@ def test_recorded_wait_errors_are_taken_one_by_one(tmp_path):
         w[i] = 1
     assert [l.take(w) for _ in range(n + 1)] == list(range(n)) + [-1]
     assert list(w) == [0] * n
+
+
+def test_every_entry_point_reports_a_wait_that_gave_up_before():
+    """Wrappers never call sb_stream_sync: without this, outputs would be wrong in silence."""
+    lib = N.lib()
+    path = [l.split()[-1] for l in open("/proc/self/maps") if l.rstrip().endswith("libscryb200.so")][0]
+    base = min(int(l.split("-")[0], 16) for l in open("/proc/self/maps") if l.rstrip().endswith("libscryb200.so"))
+    at = [l.split()[0] for l in subprocess.run(["nm", path], capture_output=True, text=True, check=True).stdout.splitlines() if "g_wait_errors" in l and "g_wait_errors_mu" not in l]
+    assert len(at) == 1
+    place = C.c_void_p.from_address(base + int(at[0], 16))
+    words, before = (C.c_uint * 16)(), place.value
+    calls = [lambda: lib.sb_kv_append(0, 0, 0, 0, 0, 0, 0, 0, 1, 1, 0, 0, 0, 0, 0, 0, 0, 0, 1.0, 0, 0), lambda: lib.sb_kv_commit(0, 1, 0, 0, 1, 0, 0),
+             lambda: lib.sb_kv_read(0, 1, 0, 1, 0, 0, 0, 0), lambda: lib.sb_tree_attention(0, 0, 0, 0, 1, 1, 1, 0, 0, 0, 0, 1, 0, 0),
+             lambda: lib.sb_verify_drafts(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, 1, 1, 1.0, 0, 0, 0, 0)]
+    place.value = C.addressof(words)
+    try:
+        for call in calls:
+            words[0] = 1
+            with pytest.raises(N.SbError, match="timed out"):
+                N.check(call())
+            assert words[0] == 0
+            with pytest.raises(N.SbError) as e:  # its own null pointers, from now on
+                N.check(call())
+            assert "timed out" not in str(e.value)
+    finally:
+        place.value = before
