@@ -307,3 +307,84 @@ torch.cuda.synchronize()
 assert bool((out == 3.0).all()), out
 """
     subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+
+
+# ---------------------------------------------------------------------------
+# streams and graphs
+
+def _step_inputs(g, b, t, v):
+    x = dict(logits=torch.randn(b, t, v, generator=g, device="cuda") * 2, parents=ints(parents_of(t)), u=torch.rand(b, t, generator=g, device="cuda"),
+             noise=noise_of(g, b, v), qkv=torch.randn(b, t, 8, 64, generator=g, device="cuda"))
+    best = x["logits"].topk(3, -1).indices
+    x["tokens"] = torch.zeros(b, t, dtype=torch.int32, device="cuda")
+    for i in range(1, t):
+        x["tokens"][:, i] = best[:, (i - 1) // 3, (i - 1) % 3].int()
+    return x
+
+
+def _step(x, cache, cl):
+    """Append, attention, verification, commit and read of one step."""
+    q, k, v = x["qkv"].split([4, 2, 2], 2)
+    q = E.kv_append(cache, k, v, cl, q=q, rope=x["rope"], q_scale=0.125)
+    y = E.tree_attention(q, cache, cl, 400, mask=x["mask"])
+    path, keep, nxt = E.verify_drafts(x["logits"], x["tokens"], x["parents"], x["u"], x["noise"], temperature=0.9)
+    E.kv_commit(cache, cl, path, keep)
+    return (y, path, keep, nxt) + E.kv_read(cache, 20, start=cl)
+
+
+def _step_setup(seed, b, t, v):
+    g = gen(seed)
+    x = _step_inputs(g, b, t, v)
+    x["rope"] = rope_tables(400, 64)
+    x["mask"] = torch.from_numpy(E.tree_mask(parents_of(t))).cuda()
+    return x, make_cache(g, b, 400, 2, 64, 16, "int8"), ints([300 - 20 * i for i in range(b)])
+
+
+@pytest.mark.parametrize("b,t,v", [(2, 13, 5000), (3, 13, 128256), (12, 20, 33001)])
+def test_a_step_on_several_streams(b, t, v):
+    """Steps of different sequences on two streams at once are what they are one after the other."""
+    steps = [_step_setup(s, b, t, v) for s in range(2)]
+    start = [[c.k.clone(), c.v.clone(), c.k_scale.clone(), c.v_scale.clone()] for _, c, _ in steps]
+    want = [_step(*s) for s in steps]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        for (x, c, cl), old in zip(steps, start):
+            for dst, src in zip((c.k, c.v, c.k_scale, c.v_scale), old):
+                dst.copy_(src)
+        torch.cuda.synchronize()
+        got = []
+        for s, stream in zip(steps, streams):
+            with torch.cuda.stream(stream):
+                got.append(_step(*s))
+        torch.cuda.synchronize()
+        for a, c in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, c))
+
+
+@pytest.mark.parametrize("b,t,v", [(2, 13, 5000), (3, 13, 128256), (12, 20, 33001)])
+def test_a_step_in_a_graph(b, t, v):
+    """A captured step, replayed on new inputs in the same tensors, is the step called directly."""
+    x, cache, cl = _step_setup(5, b, t, v)
+    parts = (cache.k, cache.v, cache.k_scale, cache.v_scale)
+    old = [p.clone() for p in parts]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        _step(x, cache, cl)  # its workspaces
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out = _step(x, cache, cl)
+    for seed in (6, 7):
+        new = _step_inputs(gen(seed), b, t, v)
+        for name in new:
+            x[name].copy_(new[name])
+        for p, o in zip(parts, old):
+            p.copy_(o)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [y.clone() for y in out] + [p.clone() for p in parts]
+        for p, o in zip(parts, old):
+            p.copy_(o)
+        want = list(_step(x, cache, cl)) + list(parts)
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
