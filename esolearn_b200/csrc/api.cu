@@ -793,7 +793,7 @@ sb_status sb_verify_drafts(const float *logits, int64_t logits_ld, const int32_t
                            const float *noise, int64_t noise_ld, int B, int N, int V, float temperature,
                            int32_t *path, int32_t *n_accept, int32_t *next, void *stream) {
     SB_TRY(wait_error_check());
-    SB_CHECK(!std::isnan(temperature), SB_ERR_ARG, "sb_verify_drafts: temperature is NaN");
+    SB_CHECK(temperature < INFINITY, SB_ERR_ARG, "sb_verify_drafts: temperature %g", (double)temperature);  // (nor NaN)
     SB_CHECK(B >= 0 && N >= 1 && N <= VERIFY_MAX_NODES && V >= 1, SB_ERR_SHAPE, "sb_verify_drafts: B %d, N %d, V %d", B, N, V);
     if (B == 0) return SB_OK;
     const bool greedy = temperature < 1e-8f;

@@ -267,12 +267,12 @@ sb_status sb_tree_attention(const sb_kv_cache *cache, const void *q, int dtype, 
  * nothing is left): a draw from w / W.  u: [B][N] uniform in [0, 1), entry i for
  * node i; noise: [B] rows of V exponential(1) numbers > 0 (stride noise_ld).
  * The accepted tokens and the next one are then distributed as sampling from
- * the target token by token.  temperature < 1e-8 is greedy: the child equal to
- * the argmax (ties -> last index, as sb_argmax_rows) is accepted; u, noise and
- * draft_probs are not read and may be NULL.  path: [B][N] accepted nodes from
- * node 0 on, then -1; n_accept: [B] their number (>= 1); next: [B].  NaN logits
- * give unspecified tokens.  N <= 1024, V <= 750000.  Uses a library-owned
- * workspace per device and stream. */
+ * the target token by token.  temperature is finite; < 1e-8 is greedy: the
+ * child equal to the argmax (ties -> last index, as sb_argmax_rows) is accepted;
+ * u, noise and draft_probs are not read and may be NULL.  path: [B][N] accepted
+ * nodes from node 0 on, then -1; n_accept: [B] their number (>= 1); next: [B].
+ * NaN logits give unspecified tokens.  N <= 1024, V <= 750000.  Uses a
+ * library-owned workspace per device and stream. */
 sb_status sb_verify_drafts(const float *logits, int64_t logits_ld, const int32_t *tokens, const int32_t *parents,
                            int parents_ld, const float *draft_probs, int64_t draft_ld, const float *u,
                            const float *noise, int64_t noise_ld, int B, int N, int V, float temperature,

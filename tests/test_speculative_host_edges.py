@@ -105,3 +105,11 @@ def test_every_entry_point_reports_a_wait_that_gave_up_before():
             assert "timed out" not in str(e.value)
     finally:
         place.value = before
+
+
+@pytest.mark.parametrize("temperature", [float("inf"), float("nan")])
+def test_temperatures_that_are_none_are_refused(temperature):
+    """An infinite temperature would turn a masked logit (-inf) into a NaN exponent; refused before any launch."""
+    args = [256, 8, 256, 256, 0, 0, 0, 256, 256, 8, 1, 2, 8, temperature, 256, 256, 256, 0]
+    with pytest.raises(N.SbError, match="temperature"):
+        N.check(N.lib().sb_verify_drafts(*args))
