@@ -108,7 +108,8 @@ static int workspace_get(int kind, size_t bytes, void **out, cudaStream_t st) {
 // statistics), one per device and stream, so that calls on different streams
 // never share it.  A buffer that is too small is replaced by one at least twice
 // its size and kept until the process ends: launches already queued, and
-// captured graphs, may still hold it.
+// captured graphs, may still hold it.  (cudaMalloc is no work of any stream, and
+// a capture that the thread's stream is in does not mind it in relaxed mode.)
 static int stream_workspace(size_t bytes, void **out, cudaStream_t st) {
     struct Entry {
         int dev;
@@ -135,7 +136,10 @@ static int stream_workspace(size_t bytes, void **out, cudaStream_t st) {
     if (e->bytes < bytes) {
         const size_t n = std::max(bytes, 2 * e->bytes);
         void *p = nullptr;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        SB_CUDA_TRY(cudaThreadExchangeStreamCaptureMode(&mode));
         const cudaError_t rc = cudaMalloc(&p, n);
+        cudaThreadExchangeStreamCaptureMode(&mode);
         if (rc != cudaSuccess) {
             cudaGetLastError();
             return set_error(SB_ERR_OOM, "workspace cudaMalloc(%zu): %s", n, cudaGetErrorString(rc));

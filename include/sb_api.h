@@ -246,9 +246,10 @@ sb_status sb_kv_read(const sb_kv_cache *cache, int B, const int32_t *start, int 
  * known to the host; it only decides how the work is split.  A token that
  * sees nothing, or does not exist, gives zeros; what a token does not see has
  * no influence on it, whatever its value.  Uses a library-owned workspace per
- * device and stream: make one call of the largest size before capturing, and
- * let a stream's calls end before it is destroyed (its handle, and with it the
- * workspace, may be given to the next one). */
+ * device and stream, of which a captured graph keeps what it was captured with:
+ * let no graph run beside calls on the stream it was captured on, nor beside
+ * another graph captured there, and let a stream's calls end before it is
+ * destroyed (its handle, and with it the workspace, may be given to the next). */
 sb_status sb_tree_attention(const sb_kv_cache *cache, const void *q, int dtype, int64_t q_stride, int B, int T,
                             int n_heads, const int32_t *ctx_len, const int32_t *n_new, const uint64_t *mask,
                             int64_t mask_ld, int max_ctx, void *out, void *stream);
@@ -271,8 +272,8 @@ sb_status sb_tree_attention(const sb_kv_cache *cache, const void *q, int dtype, 
  * child equal to the argmax (ties -> last index, as sb_argmax_rows) is accepted;
  * u, noise and draft_probs are not read and may be NULL.  path: [B][N] accepted
  * nodes from node 0 on, then -1; n_accept: [B] their number (>= 1); next: [B].
- * NaN logits give unspecified tokens.  N <= 1024, V <= 750000.  Uses a
- * library-owned workspace per device and stream. */
+ * NaN logits give unspecified tokens.  N <= 1024, V <= 750000.  The workspace is
+ * that of sb_tree_attention. */
 sb_status sb_verify_drafts(const float *logits, int64_t logits_ld, const int32_t *tokens, const int32_t *parents,
                            int parents_ld, const float *draft_probs, int64_t draft_ld, const float *u,
                            const float *noise, int64_t noise_ld, int B, int N, int V, float temperature,

@@ -312,6 +312,32 @@ assert bool((out == 3.0).all()), out
 # ---------------------------------------------------------------------------
 # streams and graphs
 
+def test_first_calls_with_workspaces_inside_a_capture():
+    # torch captures on a stream of its own, where no call has been made: split attention and verification both need room
+    code = """
+import torch, esolearn_b200 as E
+cache = E.KvCache.zeros(1, 4096, 2, 128)
+g = torch.Generator("cuda").manual_seed(0)
+cache.k.random_(-127, 128, generator=g), cache.v.random_(-127, 128, generator=g)
+cache.k_scale.fill_(0.01), cache.v_scale.fill_(0.01)
+q = torch.randn(1, 4, 8, 128, generator=g, device="cuda") * 0.1
+cl = torch.full((1,), 4000, dtype=torch.int32, device="cuda")
+logits = torch.randn(1, 4, 32000, generator=g, device="cuda")
+tokens = logits.argmax(-1).roll(1, 1).int().contiguous()
+parents = torch.tensor([-1, 0, 1, 2], dtype=torch.int32, device="cuda")
+u, noise = torch.rand(1, 4, generator=g, device="cuda"), torch.rand(1, 32000, generator=g, device="cuda") + 0.1
+run = lambda: (E.tree_attention(q, cache, cl, 4004),) + E.verify_drafts(logits, tokens, parents, u, noise)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, run()))
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
+
+
 def _step_inputs(g, b, t, v):
     x = dict(logits=torch.randn(b, t, v, generator=g, device="cuda") * 2, parents=ints(parents_of(t)), u=torch.rand(b, t, generator=g, device="cuda"),
              noise=noise_of(g, b, v), qkv=torch.randn(b, t, 8, 64, generator=g, device="cuda"))
