@@ -12,11 +12,11 @@
 // Warps work alone: a warp streams tiles of PW positions through its own ring
 // (boxes of the tensor copy engine and an mbarrier per stage; single 16-byte
 // copies where pages are not a multiple of 8 positions), keeps q's fragments, S, the sums and O in
-// registers, and takes every fourth tile of its CTA's share of the context.  A
-// reference maximum serves until a score exceeds it by 2^8 (a vote, no
-// reduction), so the steady state has no shuffles; probabilities up to 2^8 still
-// fit the f16 terms, which are scaled to at most 2^15.  Warps and then splits are
-// joined in order.
+// registers, and takes every fourth or sixth tile of its CTA's share of the
+// context.  A row's reference maximum serves until a score exceeds it by 2^8 (a
+// vote, no reduction), so the steady state has no shuffles; probabilities up to
+// 2^8 still fit the f16 terms, which are scaled to at most 2^15.  Warps and then
+// splits are joined in order.
 //
 // Tiles lie as the boxes leave them, 16-byte chunks of 128-byte rows XOR-ed with
 // the row's lowest three bits.  Both fragment loads are free of bank conflicts
@@ -25,17 +25,19 @@
 // load's phase differ where they have to (tr_position, tr_chunk).  (Rows of 64
 // bytes, int8 of head_dim 64, keep two-way conflicts.)
 //
-// Bound by instructions and their latency: about 1000 of them per 32 positions and
-// 8 rows, half of which turn codes into f16 operands, at 3 warps per scheduler.
-// 32 sequences x 1 token at 2048 positions, 8 kv heads of 4 query heads, int8: 37 us
-// (3.8 TB/s; 44 us with four warps per CTA and 16-byte copies).  26 tokens at 1100,
-// 32 kv heads, bf16: 23 us, of which the products of three terms take most.
+// Bound by latency: a warp's products, softmax and products follow one another, and
+// an SM has room for 8 to 12 warps.  Its issue slots are 47 % busy (int8, 8 rows:
+// about 1000 instructions per 32 positions, half of which turn codes into f16
+// operands) and 22 % (bf16, 32 rows, 255 registers a thread).  32 sequences x 1 token
+// at 2048 positions, 8 kv heads of 4 query heads, int8: 37 us (3.8 TB/s; 44 us with
+// four warps per CTA and 16-byte copies).  26 tokens at 1100, 32 kv heads, bf16: 24 us.
 //
 // Up to 32 rows, beyond which it would read the cache twice.  With 32 rows this
-// kernel and the 128-row one take, in us, for 8 sequences at 2000: 32 kv heads, int8
-// 93 and 135, bf16 116 and 137; 8 kv heads, int8 33 and 38, bf16 42 and 48.  For one
-// sequence of 8 kv heads at 2000 they are level with int8 (18 both; 8000: 25, 24), and
-// the other is ahead with bf16 (20 and 17; 8000: 29 and 25).
+// kernel and the 128-row one take, in us, f32 q, for 8 sequences at 2000: 32 kv heads,
+// int8 95 and 131, bf16 118 and 143; 8 kv heads, int8 35 and 37, bf16 42 and 48.  For
+// one sequence at 2000 the other is ahead: 32 kv heads, int8 26 and 24, bf16 29 and 26;
+// 8 kv heads, int8 19 and 16, bf16 21 and 18 (bf16 q: 25 and 20, 19 and 16).  With 8
+// rows this one is ahead throughout: 32 kv heads at 2000, one sequence, 14 and 23.
 #include "attention_tree.cuh"
 
 #include <cuda_fp16.h>

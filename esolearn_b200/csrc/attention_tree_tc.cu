@@ -38,12 +38,14 @@
 // matrices) took 39 clocks per warp instruction.
 //
 // A tile's products take 1536 clocks (bf16 cache, bf16 q) or 2048 (int8, f32 q: its
-// 10,000 warp instructions also take 2600 issue slots per scheduler), yet it takes
+// 10,600 warp instructions also take 2700 issue slots per scheduler), yet it takes
 // 4000 and 5000: the chain scores - softmax - p V - sums of a tile, of which too
-// little runs under the next one's, and the shared schedulers bound it.  (Looking
-// pages and scales up a tile further ahead cost 10 %: more instructions.)  512 tokens behind 8192, 8 kv heads of 4, bf16: 135 to 144 us (500
-// TFLOP/s, each product counted once); 32 tokens x 8 sequences up to 4096, 8 kv heads
-// of 8, int8, f32: 111 to 121 us (290 TFLOP/s).
+// little runs under the next one's, and the shared schedulers bound it (tensor cores
+// 45 % and 31 % busy, issue slots 43 % and 45 %).  Looking pages and scales up a tile
+// further ahead cost 10 %: more instructions.  512 tokens behind 8192, 8 kv heads of
+// 4, bf16: 136 to 144 us (490 TFLOP/s, each product counted once), with f32 q 201 to
+// 221; 32 tokens x 8 sequences up to 4096, 8 kv heads of 8, int8, f32 q: 113 to 125 us
+// (290 TFLOP/s).
 #include "attention_tree.cuh"
 
 #include <algorithm>
@@ -60,9 +62,9 @@ namespace {
 constexpr int TT_THREADS = 512, TT_ROWS = 128, TT_TILE = 128;
 constexpr int TT_SOFTMAX_WARPS = 8, TT_LOADERS = 3, TT_LOAD0 = 12, TT_MMA = 15;
 // Registers of a thread, 128 at launch: 2 * softmax + sums + (loaders and products) = 4 * 128.  What they save is
-// spills, and which role gains from more differs: 512 tokens behind 8192, bf16 cache and q, take 142 us with 144, 152
-// and 72 and 134.5 with 152, 152 and 56, which costs a bf16 cache with f32 q 2 %; 256 rows x 8 sequences at 2000, int8,
-// take 311 us with 144, 152 and 72 and 306 with 144, 160 and 64.
+// spills, and which role gains from more differs: 512 tokens behind 8192, bf16 cache and q, take 140 to 150 us with 144,
+// 152 and 72 and 139 with 152, 152 and 56, which leaves a bf16 cache with f32 q as it is (214 both); 256 rows x 8
+// sequences at 2000, 8 kv heads, int8, take 68.7 us with 144, 152 and 72 and 68.1 with 144, 160 and 64.
 constexpr int tt_regs_softmax(int dt, bool bf16) { return dt != SB_KV_I8 && bf16 ? 152 : 144; }
 constexpr int tt_regs_sums(int dt) { return dt == SB_KV_I8 ? 160 : 152; }
 constexpr int tt_regs_rest(int dt, bool bf16) { return 4 * 128 - 2 * tt_regs_softmax(dt, bf16) - tt_regs_sums(dt); }

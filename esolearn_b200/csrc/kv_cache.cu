@@ -1,10 +1,11 @@
 // Writing, moving and reading rows of a paged K/V cache (kv_cache.cuh).
 //
-// Quantised rows follow quantize_symmetric's rule (quantize.rs:16-32) row by row,
-// in f32 without contraction: scale = max|x| * (1 / 127), code = x * (1 / scale)
-// rounded half away from zero and held to [-127, 127].  The scale is a product, as
-// tensor programs evaluate a division by a constant, so that rows agree with theirs
-// bit for bit; it lies within one unit in the last place of max|x| / 127.
+// Quantised rows follow quantize_symmetric's rule (quantize.rs:16-32) row by row, in
+// f32 without contraction, but for their scale: scale = max|x| * (1 / 127), code =
+// x * (1 / scale) rounded half away from zero and held to [-127, 127].
+// quantize_symmetric divides by 127; the product is what tensor programs make of a
+// division by a constant, so that rows agree with theirs bit for bit, and lies
+// within one unit in the last place of the quotient.
 #include "kv_cache.cuh"
 
 #include <algorithm>
@@ -54,9 +55,10 @@ constexpr int APPEND_THREADS = 256;
 // A lane holds 16 bytes of a head's row, a group of lanes the whole row; a group
 // takes HEADS heads of a (b, t) row (q heads first, then k, then v), so that
 // their loads are in flight together and the row's cos and sin are read once.
-// Bound by memory, with a third of the issue slots taken: 4096 rows of 64 + 2 * 8
-// heads of 128, f32 to int8, 310 MB in 64 us (4.8 TB/s).  Rows looped over with
-// the next one's loads ahead took 78 us, eight heads a group 90.
+// Bound by memory, with 62 % of the issue slots taken: 4096 rows of 64 + 2 * 8
+// heads of 128, f32 to int8, 310 MB in 62 us (5.0 TB/s); to bf16 54 us (5.9 TB/s),
+// to f32 55 us (6.1 TB/s).  Rows looped over with the next one's loads ahead took
+// 78 us to int8, eight heads a group 90.
 template <int HD, bool BF16>
 struct Append {
     static constexpr int E = Io<BF16>::E;

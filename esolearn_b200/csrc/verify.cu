@@ -453,12 +453,12 @@ __global__ void __launch_bounds__(VT, 1) verify_kernel(const VerifyArgs a, int t
 // steps, of about 4 us each (all rows of 1e8 bytes take 30 us).  With the draft's
 // probabilities walks are long, since its tokens are mostly accepted.  Walk against
 // all rows first, in us, V 128256 where not said:
-//   chains with probabilities: 1 x 6 nodes, V 32000: 21.6, 9.9; 16 x 6, V 32000:
-//     25.4, 11.8; 8 x 9 (3.7e7 bytes): 44, 22;
-//   given tokens: 1 x 2, V 32000: 10.5, 9.5; 8 x 2: 14.0, 12.8; 32 x 2 (3.3e7 bytes):
-//     23.6, 22.7; 4 x 26 (5.3e7): 22.4, 25.1; 32 x 6 (9.9e7): 28.8, 37.6;
-//     32 x 26 (4.3e8): 34.7, 84;
-//   a single node: the same within 0.3.
+//   chains with probabilities: 1 x 6 nodes, V 32000: 21.5, 10.0; 16 x 6, V 32000:
+//     25.6, 12.1; 8 x 9 (3.7e7 bytes): 45, 21.5;
+//   given tokens: 1 x 2, V 32000: 10.8, 9.8; 8 x 2: 14.2, 13.0; 32 x 2 (3.3e7 bytes):
+//     23.4, 23.2; 4 x 26 (5.3e7): 22.5, 25.5; 32 x 6 (9.9e7): 28.9, 38.0;
+//     32 x 26 (4.3e8): 34.7, 85;
+//   a single node: 10.4, 9.9; 8 of them 10.6, 11.2.
 bool verify_all_rows(const VerifyArgs &a) {
     return a.temperature >= 1e-8f && a.N > 1 && (double)a.B * a.N * a.V * 4 < (a.draft ? 1.0e8 : 4.0e7);
 }

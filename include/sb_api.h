@@ -213,8 +213,9 @@ typedef struct sb_kv_cache {
  * t], or t when depth is NULL (depth_ld 0: one row for all sequences).  q is
  * then multiplied by q_scale and stored to q_out [B][T][n_heads][head_dim]
  * (n_heads 0: no q).  SB_KV_I8 rows follow the rule of quantize_symmetric
- * (quantize.rs:16-32) row by row, in f32: scale = max|x| * (1/127), codes x *
- * (1/scale) rounded half away from zero.
+ * (quantize.rs:16-32) row by row, in f32, but for the scale, which is a product:
+ * scale = max|x| * (1/127) (within one unit in the last place of the quotient),
+ * codes x * (1/scale) rounded half away from zero.
  * Row (b, t) of q, k, v starts at (b*T + t) * its stride (in elements, a
  * multiple of 4 for f32 and 8 for bf16), its heads contiguous, so all three
  * may lie in one fused q|k|v projection.  dtype (SB_DTYPE_F32 or SB_DTYPE_BF16)
@@ -268,7 +269,8 @@ sb_status sb_tree_attention(const sb_kv_cache *cache, const void *q, int dtype, 
  * nothing is left): a draw from w / W.  u: [B][N] uniform in [0, 1), entry i for
  * node i; noise: [B] rows of V exponential(1) numbers > 0 (stride noise_ld).
  * The accepted tokens and the next one are then distributed as sampling from
- * the target token by token.  temperature is finite; < 1e-8 is greedy: the
+ * the target token by token.  (Top-k or top-p sampling: set the logits outside
+ * the choice to -inf before the call.)  temperature is finite; < 1e-8 is greedy: the
  * child equal to the argmax (ties -> last index, as sb_argmax_rows) is accepted;
  * u, noise and draft_probs are not read and may be NULL.  path: [B][N] accepted
  * nodes from node 0 on, then -1; n_accept: [B] their number (>= 1); next: [B].
